@@ -20,6 +20,7 @@ import torch.nn as nn
 from ..ops import functional as O
 from .layers import (DepthwiseConv2d, PointwiseConv2d, StemConv2d,
                      create_conv2d, drop_path, sigmoid)
+from .layers_extra import GroupNorm2d
 
 __all__ = [
     "BN_MOMENTUM_TF_DEFAULT",
@@ -143,7 +144,7 @@ class ConvBnAct(nn.Module):
         self.bn1 = norm_layer(out_chs, **norm_kwargs)
         self.act1 = act_layer(inplace=True)
         self._act_name = O.act_name_of(self.act1)
-        _mark_bn_producer(self.conv)
+        _mark_bn_producer(self.conv, norm_layer)
 
     def feature_module(self, location):
         return "act1"
@@ -153,20 +154,30 @@ class ConvBnAct(nn.Module):
 
     def forward(self, x):
         x = self.conv(x)
-        if self._act_name != "other" and O.fusable_bn(self.bn1):
+        if self._act_name != "other" and _fuses(self.bn1, self.act1):
             return O.bn_act(x, self.bn1, self._act_name)
         return self.act1(self.bn1(x))
 
 
-def _mark_bn_producer(conv):
+def _mark_bn_producer(conv, norm_layer=nn.BatchNorm2d):
     """Ask a conv whose output feeds a fused BatchNorm to emit the BN stats
-    from its epilogue — the BN then skips its own stats pass over y."""
+    from its epilogue — the BN then skips its own stats pass over y. A group
+    norm has statistics of each image instead and reads none of these."""
+    if getattr(norm_layer, "func", norm_layer) is GroupNorm2d:
+        return
     if isinstance(conv, (PointwiseConv2d, DepthwiseConv2d, StemConv2d)):
         conv.emit_bn_stats = True
 
 
+def _fuses(norm, act_module):
+    """Whether bn_act takes this norm with this activation. A group norm is
+    not fused with ReLU6: the fused relu has no upper bound."""
+    return O.fusable_bn(norm) or (
+        O.fusable_gn(norm) and not isinstance(act_module, nn.ReLU6))
+
+
 def _bn_act(bn, act_module, act_name, x, residual=None, drop_path_mask=None):
-    if act_name != "other" and O.fusable_bn(bn):
+    if act_name != "other" and _fuses(bn, act_module):
         return O.bn_act(x, bn, act_name, residual, drop_path_mask)
     y = act_module(bn(x))
     if drop_path_mask is not None:
@@ -204,7 +215,7 @@ class DepthwiseSeparableConv(nn.Module):
         self.conv_dw = create_conv2d(
             in_chs, in_chs, dw_kernel_size, stride=stride, dilation=dilation,
             padding=pad_type, depthwise=True)
-        _mark_bn_producer(self.conv_dw)
+        _mark_bn_producer(self.conv_dw, norm_layer)
         self.bn1 = norm_layer(in_chs, **norm_kwargs)
         self.act1 = act_layer(inplace=True)
 
@@ -215,7 +226,7 @@ class DepthwiseSeparableConv(nn.Module):
             self.se = None
 
         self.conv_pw = create_conv2d(in_chs, out_chs, pw_kernel_size, padding=pad_type)
-        _mark_bn_producer(self.conv_pw)
+        _mark_bn_producer(self.conv_pw, norm_layer)
         self.bn2 = norm_layer(out_chs, **norm_kwargs)
         self.act2 = act_layer(inplace=True) if self.has_pw_act else nn.Identity()
         self._act_name = O.act_name_of(self.act1)
@@ -265,14 +276,14 @@ class InvertedResidual(nn.Module):
         self.drop_path_rate = drop_path_rate
 
         self.conv_pw = create_conv2d(in_chs, mid_chs, exp_kernel_size, padding=pad_type, **conv_kwargs)
-        _mark_bn_producer(self.conv_pw)
+        _mark_bn_producer(self.conv_pw, norm_layer)
         self.bn1 = norm_layer(mid_chs, **norm_kwargs)
         self.act1 = act_layer(inplace=True)
 
         self.conv_dw = create_conv2d(
             mid_chs, mid_chs, dw_kernel_size, stride=stride, dilation=dilation,
             padding=pad_type, depthwise=True, **conv_kwargs)
-        _mark_bn_producer(self.conv_dw)
+        _mark_bn_producer(self.conv_dw, norm_layer)
         self.bn2 = norm_layer(mid_chs, **norm_kwargs)
         self.act2 = act_layer(inplace=True)
 
@@ -283,7 +294,7 @@ class InvertedResidual(nn.Module):
             self.se = None
 
         self.conv_pwl = create_conv2d(mid_chs, out_chs, pw_kernel_size, padding=pad_type, **conv_kwargs)
-        _mark_bn_producer(self.conv_pwl)
+        _mark_bn_producer(self.conv_pwl, norm_layer)
         self.bn3 = norm_layer(out_chs, **norm_kwargs)
         self._act_name = O.act_name_of(self.act1)
 
@@ -393,7 +404,7 @@ class EdgeResidual(nn.Module):
 
         self.conv_pwl = create_conv2d(
             mid_chs, out_chs, pw_kernel_size, stride=stride, dilation=dilation, padding=pad_type)
-        _mark_bn_producer(self.conv_pwl)
+        _mark_bn_producer(self.conv_pwl, norm_layer)
         self.bn2 = norm_layer(out_chs, **norm_kwargs)
         self._act_name = O.act_name_of(self.act1)
 

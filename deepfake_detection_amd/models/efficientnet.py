@@ -19,7 +19,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops import functional as O
-from .blocks import resolve_bn_args, round_channels
+from .blocks import _fuses, resolve_bn_args, round_channels
 from .builder import EfficientNetBuilder, decode_arch_def, efficientnet_init_weights
 from .helpers import load_pretrained
 from .layers import SelectAdaptivePool2d, Swish, create_conv2d
@@ -123,8 +123,8 @@ class EfficientNet(nn.Module):
         # Head
         self.conv_head = create_conv2d(self._in_chs, self.num_features, 1, padding=pad_type)
         from .blocks import _mark_bn_producer as _mark
-        _mark(self.conv_head)
-        _mark(self.conv_stem)
+        _mark(self.conv_head, norm_layer)
+        _mark(self.conv_stem, norm_layer)
         self.bn2 = norm_layer(self.num_features, **norm_kwargs)
         self.act2 = act_layer(inplace=True)
         self.global_pool = SelectAdaptivePool2d(pool_type=global_pool)
@@ -151,13 +151,13 @@ class EfficientNet(nn.Module):
 
     def forward_features(self, x):
         x = self.conv_stem(x)
-        if self._act_name != "other" and O.fusable_bn(self.bn1):
+        if self._act_name != "other" and _fuses(self.bn1, self.act1):
             x = O.bn_act(x, self.bn1, self._act_name)
         else:
             x = self.act1(self.bn1(x))
         x = self.blocks(x)
         x = self.conv_head(x)
-        if self._act_name != "other" and O.fusable_bn(self.bn2):
+        if self._act_name != "other" and _fuses(self.bn2, self.act2):
             x = O.bn_act(x, self.bn2, self._act_name)
         else:
             x = self.act2(self.bn2(x))

@@ -16,11 +16,14 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops import functional as O
 from .layers import get_padding, pad_same
 
 __all__ = [
     "SplitBatchNorm2d",
     "convert_splitbn_model",
+    "GroupNorm2d",
+    "convert_groupnorm_model",
     "SEModule",
     "EcaModule",
     "CecaModule",
@@ -90,6 +93,41 @@ def convert_splitbn_model(module, num_splits=2):
         mod.add_module(name, convert_splitbn_model(child, num_splits=num_splits))
     del module
     return mod
+
+
+class GroupNorm2d(nn.GroupNorm):
+    """GroupNorm of image batches in the place of a BatchNorm2d: it takes the
+    same arguments where a model builds its norms (``momentum`` has no meaning
+    here and is ignored).
+
+    gcd(num_features, num_groups) groups, so that any number of channels can be
+    split: 32 of them at the default for most widths. Runs the fused kernels of
+    ops.functional.group_norm_act on the GPU; blocks that fuse their activation
+    call that op with this module directly.
+    """
+
+    def __init__(self, num_features, eps=1e-5, momentum=None, affine=True, num_groups=32):
+        super().__init__(math.gcd(num_features, num_groups), num_features, eps, affine)
+
+    def forward(self, x):
+        return O.group_norm_act(x, self, "none")
+
+
+def convert_groupnorm_model(module, num_groups=32):
+    """Replace every BatchNorm2d by a GroupNorm2d that keeps its eps and its
+    weight and bias; running statistics are dropped. Returns the model."""
+    if type(module) is nn.BatchNorm2d:
+        mod = GroupNorm2d(module.num_features, module.eps, affine=module.affine,
+                          num_groups=num_groups)
+        mod.train(module.training)
+        if module.affine:
+            mod.weight, mod.bias = module.weight, module.bias
+        return mod
+    if getattr(module, "emit_bn_stats", False):
+        module.emit_bn_stats = False  # no BatchNorm reads them any more
+    for name, child in module.named_children():
+        setattr(module, name, convert_groupnorm_model(child, num_groups))
+    return module
 
 
 class SEModule(nn.Module):

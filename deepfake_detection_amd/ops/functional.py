@@ -8,7 +8,8 @@ arrives and the extension is missing, we raise (see ops/extension.py).
 import torch
 import torch.nn.functional as F
 
-from .extension import gpu_ops_required
+from . import reference
+from .extension import gpu_ops_required, load_extension
 
 _FUSED_ACTS = ("none", "relu", "silu")
 
@@ -48,8 +49,10 @@ def bn_act(x, bn, act: str = "silu", residual=None, drop_path_mask=None):
 
     drop_path_mask: fp32 [B] per-sample 0-or-1/keep values (stochastic
     depth, reference drop.py:84-100), applied to the BN+act output before
-    the residual add."""
+    the residual add. A GroupNorm2d in bn's place runs as group_norm_act."""
     if not fusable_bn(bn):
+        if fusable_gn(bn) and act in _FUSED_ACTS:
+            return group_norm_act(x, bn, act, residual, drop_path_mask)
         # Subclass with its own semantics (SplitBatchNorm2d, SyncBatchNorm...):
         # module dispatch, then the named activation.
         y = bn(x)
@@ -110,6 +113,54 @@ def bn_act(x, bn, act: str = "silu", residual=None, drop_path_mask=None):
     if residual is not None:
         y = y + residual
     return y
+
+
+def fusable_gn(norm) -> bool:
+    """True for GroupNorm2d, whose forward is the fused op itself; subclasses
+    and other group norms keep their own forward."""
+    from ..models.layers_extra import GroupNorm2d
+
+    return type(norm) is GroupNorm2d
+
+
+def fusable_norm(norm) -> bool:
+    """True for the norms that bn_act runs fused with its activation."""
+    return fusable_bn(norm) or fusable_gn(norm)
+
+
+def group_norm_act(x, gn, act: str = "silu", residual=None, drop_path_mask=None):
+    """GroupNorm + activation (+ fused drop_path scale and residual add) of a
+    [B, C, H, W] image batch: act(gn(x)) * drop_path_mask + residual.
+
+    The statistics are of one image each, so neither the batch's size nor the
+    other images change an image's result, in training and in eval alike.
+    GPU: HIP kernels (ops/hip/group_norm.hip), channels_last in and out (other
+    layouts are copied), fp32/bf16/fp16, statistics and parameter gradients in
+    fp32; differentiable once, in x, the parameters and residual. CPU: torch
+    ops of the same result.
+
+    gn: an ``nn.GroupNorm`` (its num_groups, eps, weight and bias are used).
+    act: "silu", "relu" or "none". drop_path_mask: [B] per-sample 0-or-1/keep
+    values, without a gradient, as bn_act takes them.
+    """
+    if act not in _FUSED_ACTS:
+        raise ValueError(f"group_norm_act: act must be one of {_FUSED_ACTS}, got {act!r}")
+    if x.dim() != 4:
+        raise ValueError(f"group_norm_act: [B, C, H, W] expected, got {tuple(x.shape)}")
+    if x.shape[1] != gn.num_channels:
+        raise ValueError(f"group_norm_act: {gn.num_channels} channels expected, "
+                         f"got {x.shape[1]}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"group_norm_act: residual must be {tuple(x.shape)}, "
+                         f"got {tuple(residual.shape)}")
+    if drop_path_mask is not None and drop_path_mask.shape != x.shape[:1]:
+        raise ValueError(f"group_norm_act: drop_path_mask must be ({x.shape[0]},), "
+                         f"got {tuple(drop_path_mask.shape)}")
+    if x.is_cuda and gpu_ops_required():
+        return load_extension().group_norm_act(
+            x, gn.weight, gn.bias, gn.num_groups, gn.eps, act, residual, drop_path_mask)
+    return reference.group_norm_act_forward(
+        x, gn.num_groups, gn.weight, gn.bias, gn.eps, act, residual, drop_path_mask)
 
 
 def se(x, conv_reduce, act_module, conv_expand):

@@ -54,6 +54,10 @@ std::vector<at::Tensor> head_ce_fwd(at::Tensor x, at::Tensor w, at::Tensor bias,
 std::vector<at::Tensor> head_ce_bwd(at::Tensor dloss, at::Tensor logits,
                                     at::Tensor x, at::Tensor w, at::Tensor target,
                                     double smoothing);
+at::Tensor group_norm_act(at::Tensor x, c10::optional<at::Tensor> weight,
+                          c10::optional<at::Tensor> bias, int64_t groups, double eps,
+                          std::string act, c10::optional<at::Tensor> residual,
+                          c10::optional<at::Tensor> drop_path);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "deepfake_detection_amd gfx950 (MI355X/CDNA4) kernels";
@@ -92,4 +96,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "stem conv implicit-GEMM weight grad");
   m.def("head_ce_fwd", &head_ce_fwd, "fused classifier GEMM + smoothed-CE fwd");
   m.def("head_ce_bwd", &head_ce_bwd, "fused classifier + CE backward");
+  m.def("group_norm_act", &group_norm_act,
+        "group norm + act (* drop_path) (+ residual), NHWC, differentiable",
+        py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("groups"),
+        py::arg("eps"), py::arg("act"), py::arg("residual") = py::none(),
+        py::arg("drop_path") = py::none());
 }

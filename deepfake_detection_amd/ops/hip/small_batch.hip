@@ -1,0 +1,166 @@
+// Host side of the group norm + activation op: checks, allocation, autograd.
+// The kernels are in group_norm.hip.
+
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+
+#include <string>
+
+#include "common.h"
+#include "group_norm.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<at::Tensor>;
+
+GnType gn_type(const at::Tensor& x, const char* who) {
+  switch (x.scalar_type()) {
+    case at::kFloat: return GnType::kF32;
+    case at::kBFloat16: return GnType::kBf16;
+    case at::kHalf: return GnType::kF16;
+    default:
+      TORCH_CHECK_TYPE(false, who, ": float32, bfloat16 or float16 expected, got ",
+                       x.scalar_type());
+  }
+}
+
+void check_launch(hipError_t e, const char* who) {
+  TORCH_CHECK(e == hipSuccess, who, ": ", hipGetErrorString(e));
+}
+
+const float* f32_or_null(const at::Tensor& t) {
+  return t.defined() ? t.data_ptr<float>() : nullptr;
+}
+
+struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor x, OptTensor weight_opt,
+                            OptTensor bias_opt, OptTensor residual_opt, OptTensor drop_opt,
+                            int64_t groups, double eps, int64_t act) {
+    const auto weight = weight_opt.value_or(at::Tensor()), bias = bias_opt.value_or(at::Tensor()),
+               residual = residual_opt.value_or(at::Tensor()),
+               drop = drop_opt.value_or(at::Tensor());
+    auto y = at::empty_like(x);
+    auto opts = x.options().dtype(at::kFloat);
+    auto mean = at::empty({x.size(0), groups}, opts);
+    auto rstd = at::empty({x.size(0), groups}, opts);
+    GnArgs a = args(x, weight, bias, drop, mean, rstd, groups, act);
+    a.eps = (float)eps;
+    a.residual = residual.defined() ? residual.data_ptr() : nullptr;
+    a.y = y.data_ptr();
+    if (x.numel() > 0) {
+      auto ws = at::empty({gn_fwd_ws(a)}, opts);
+      a.ws = ws.data_ptr<float>();
+      check_launch(gn_fwd(a, at::hip::getCurrentHIPStream().stream()), "group_norm_act");
+    }
+    ctx->save_for_backward({x, weight, bias, drop, mean, rstd});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["residual"] = residual.defined();
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "group_norm_act: gradients of gradients are not supported");
+    auto saved = ctx->get_saved_variables();
+    const auto &x = saved[0], &weight = saved[1], &bias = saved[2], &drop = saved[3],
+               &mean = saved[4], &rstd = saved[5];
+    const c10::DeviceGuard guard(x.device());
+    auto opts = x.options().dtype(at::kFloat);
+    at::Tensor dx, dweight, dbias, dres;
+    // the tensors that were given, in the order of forward's arguments
+    size_t input = 0;
+    if (ctx->needs_input_grad(input++)) dx = at::empty_like(x);
+    if (weight.defined() && ctx->needs_input_grad(input++)) dweight = at::empty({x.size(1)}, opts);
+    if (bias.defined() && ctx->needs_input_grad(input++)) dbias = at::empty({x.size(1)}, opts);
+    if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(input++)) dres = grads[0];
+    if (x.numel() == 0) {
+      if (dweight.defined()) dweight.zero_();
+      if (dbias.defined()) dbias.zero_();
+    } else if (dx.defined() || dweight.defined() || dbias.defined()) {
+      auto dy = grads[0].to(x.scalar_type()).contiguous(at::MemoryFormat::ChannelsLast);
+      GnArgs a = args(x, weight, bias, drop, mean, rstd,
+                      ctx->saved_data["groups"].toInt(), ctx->saved_data["act"].toInt());
+      a.dy = dy.data_ptr();
+      a.dx = dx.defined() ? dx.data_ptr() : nullptr;
+      a.dweight = dweight.defined() ? dweight.data_ptr<float>() : nullptr;
+      a.dbias = dbias.defined() ? dbias.data_ptr<float>() : nullptr;
+      auto ws = at::empty({gn_bwd_ws(a)}, opts);
+      a.ws = ws.data_ptr<float>();
+      check_launch(gn_bwd(a, at::hip::getCurrentHIPStream().stream()),
+                   "group_norm_act backward");
+    }
+    return {dx, dweight, dbias, dres, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+
+  static GnArgs args(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias,
+                     const at::Tensor& drop, const at::Tensor& mean, const at::Tensor& rstd,
+                     int64_t groups, int64_t act) {
+    GnArgs a = {};
+    a.n = x.size(0);
+    a.hw = x.size(2) * x.size(3);
+    a.c = (int)x.size(1);
+    a.groups = (int)groups;
+    a.type = gn_type(x, "group_norm_act");
+    a.act = (int)act;
+    a.x = x.data_ptr();
+    const at::Tensor& param = weight.defined() ? weight : bias;
+    a.ptype = param.defined() ? gn_type(param, "group_norm_act: parameters") : GnType::kF32;
+    a.weight = weight.defined() ? weight.data_ptr() : nullptr;
+    a.bias = bias.defined() ? bias.data_ptr() : nullptr;
+    a.drop = f32_or_null(drop);
+    a.mean = mean.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
+    return a;
+  }
+};
+
+}  // namespace
+
+at::Tensor group_norm_act(at::Tensor x, OptTensor weight_opt,
+                          OptTensor bias_opt, int64_t groups, double eps,
+                          std::string act_s, OptTensor residual_opt,
+                          OptTensor drop_opt) {
+  const char* who = "group_norm_act";
+  TORCH_CHECK(x.is_cuda() && x.dim() == 4, who, ": 4D CUDA tensor expected");
+  gn_type(x, who);
+  const int64_t c = x.size(1);
+  TORCH_CHECK(c <= INT_MAX / 2, who, ": too many channels");
+  TORCH_CHECK(groups > 0 && c % groups == 0, who, ": ", c, " channels are not a multiple of ",
+              groups, " groups");
+  Act act = Act::kNone;
+  if (act_s == "relu") act = Act::kRelu;
+  else if (act_s == "silu") act = Act::kSilu;
+  else TORCH_CHECK(act_s == "none", who, ": unknown activation '", act_s, "'");
+  auto param = [&](const OptTensor& t, const char* name) {
+    if (!t.has_value() || !t->defined()) return at::Tensor();
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == c && t->device() == x.device(), who, ": ", name,
+                " must be [", c, "] on the device of x");
+    return t->contiguous();
+  };
+  const c10::DeviceGuard guard(x.device());
+  auto weight = param(weight_opt, "weight"), bias = param(bias_opt, "bias");
+  if (weight.defined() && bias.defined() && weight.scalar_type() != bias.scalar_type()) {
+    weight = weight.to(at::kFloat);
+    bias = bias.to(at::kFloat);
+  }
+  at::Tensor residual, drop;
+  if (residual_opt.has_value() && residual_opt->defined()) {
+    TORCH_CHECK(residual_opt->sizes() == x.sizes() && residual_opt->device() == x.device(),
+                who, ": residual must have the shape and device of x");
+    residual = residual_opt->to(x.scalar_type()).contiguous(at::MemoryFormat::ChannelsLast);
+  }
+  if (drop_opt.has_value() && drop_opt->defined()) {
+    TORCH_CHECK(drop_opt->numel() == x.size(0) && drop_opt->device() == x.device(), who,
+                ": drop_path_mask must have one value for each image, on the device of x");
+    TORCH_CHECK(!drop_opt->requires_grad(), who, ": drop_path_mask has no gradient");
+    drop = drop_opt->to(at::kFloat).contiguous();
+  }
+  auto given = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; };
+  return GroupNormAct::apply(x.contiguous(at::MemoryFormat::ChannelsLast), given(weight),
+                             given(bias), given(residual), given(drop), groups, eps,
+                             (int64_t)act);
+}

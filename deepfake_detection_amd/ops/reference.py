@@ -23,6 +23,29 @@ def bn_act_forward(x, weight, bias, running_mean, running_var, training, momentu
     return ACTS[act](y)
 
 
+def group_norm_act_forward(x, num_groups, weight, bias, eps, act="silu", residual=None,
+                           drop_path=None):
+    """GroupNorm + activation, * drop_path by image, + residual, computed in
+    fp32 at least and rounded once to x's type."""
+    wide = torch.promote_types(x.dtype, torch.float32)
+    n, c = x.shape[:2]
+    v = x.to(wide).reshape(n, num_groups, -1)
+    if v.numel() > 0:
+        v = v - v.mean(dim=2, keepdim=True)
+        v = v * torch.rsqrt((v * v).mean(dim=2, keepdim=True) + eps)
+    y = v.reshape(x.shape)
+    if weight is not None:
+        y = y * weight.to(wide).view(1, c, 1, 1)
+    if bias is not None:
+        y = y + bias.to(wide).view(1, c, 1, 1)
+    y = ACTS[act](y)
+    if drop_path is not None:
+        y = y * drop_path.to(wide).view(-1, 1, 1, 1)
+    if residual is not None:
+        y = y + residual.to(wide)
+    return y.to(x.dtype)
+
+
 def se_forward(x, w_reduce, b_reduce, w_expand, b_expand, act="silu", gate="sigmoid"):
     """Squeeze-excite chain: global-avg-pool -> 1x1 reduce -> act -> 1x1
     expand -> sigmoid gate -> broadcast multiply

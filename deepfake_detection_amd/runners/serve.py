@@ -29,12 +29,16 @@ class InferenceEngine:
     """Owns the model and runs micro-batched forwards."""
 
     def __init__(self, checkpoint="", model_name="efficientnet_deepfake_v4",
-                 device=None, fp16=True, max_batch=32, batch_window_ms=3.0):
+                 device=None, fp16=True, max_batch=32, batch_window_ms=3.0, group_norm=0):
         self.device = device or ("cuda" if torch.cuda.is_available() else "cpu")
         self.dtype = torch.float16 if (fp16 and self.device == "cuda") else torch.float32
         model = create_deepfake_model_v4(
             model_name, num_classes=2, in_chans=12,
             checkpoint_path=checkpoint, strict=False)
+        if group_norm:
+            from ..models.layers_extra import convert_groupnorm_model
+
+            model = convert_groupnorm_model(model, group_norm)
         model = params.DeepFakeModel(model).to(self.device).to(self.dtype).eval()
         if self.device == "cuda":
             model = model.to(memory_format=torch.channels_last)
@@ -129,13 +133,16 @@ def main(argv=None):
     p.add_argument("--max-batch", type=int, default=32)
     p.add_argument("--batch-window-ms", type=float, default=3.0)
     p.add_argument("--no-fp16", action="store_true")
+    p.add_argument("--group-norm", type=int, default=0, metavar="G",
+                   help="the model was trained with --group-norm G")
     args = p.parse_args(argv)
 
     import uvicorn
 
     engine = InferenceEngine(
         checkpoint=args.checkpoint, model_name=args.model, fp16=not args.no_fp16,
-        max_batch=args.max_batch, batch_window_ms=args.batch_window_ms)
+        max_batch=args.max_batch, batch_window_ms=args.batch_window_ms,
+        group_norm=args.group_norm)
     uvicorn.run(create_app(engine), host=args.host, port=args.port)
 
 

@@ -20,7 +20,7 @@ from ..params import DeepFakeModel, preprocess_image
 
 
 def test_img(img_paths, checkpoint_path="../models/model_half.pth.tar",
-             device=None, dtype=None):
+             device=None, dtype=None, group_norm=0):
     if device is None:
         device = "cuda" if torch.cuda.is_available() else "cpu"
     if dtype is None:
@@ -29,6 +29,10 @@ def test_img(img_paths, checkpoint_path="../models/model_half.pth.tar",
     basemodel = create_deepfake_model_v4(
         "efficientnet_deepfake_v4", num_classes=2, in_chans=12,
         checkpoint_path=checkpoint_path, strict=False)
+    if group_norm:
+        from ..models.layers_extra import convert_groupnorm_model
+
+        basemodel = convert_groupnorm_model(basemodel, group_norm)
     model = DeepFakeModel(basemodel)
     model = model.to(device=device, dtype=dtype)
     if device == "cuda":
@@ -54,8 +58,11 @@ def main(argv=None):
     parser.add_argument("images", nargs="+", help="image paths")
     parser.add_argument("--checkpoint", default="../models/model_half.pth.tar")
     parser.add_argument("--device", default=None)
+    parser.add_argument("--group-norm", type=int, default=0, metavar="G",
+                        help="the model was trained with --group-norm G")
     args = parser.parse_args(argv)
-    test_img(args.images, checkpoint_path=args.checkpoint, device=args.device)
+    test_img(args.images, checkpoint_path=args.checkpoint, device=args.device,
+             group_norm=args.group_norm)
 
 
 if __name__ == "__main__":

@@ -136,6 +136,9 @@ def _build_parser():
     parser.add_argument("--sync-bn", action="store_true")
     parser.add_argument("--dist-bn", type=str, default="")
     parser.add_argument("--split-bn", action="store_true")
+    parser.add_argument("--group-norm", type=int, default=0, metavar="G",
+                        help="replace every BatchNorm by a group norm of at most G "
+                             "groups: results no longer depend on the batch")
     # EMA
     parser.add_argument("--model-ema", action="store_true", default=False)
     parser.add_argument("--model-ema-force-cpu", action="store_true", default=False)
@@ -221,6 +224,13 @@ def main(rank, args, args_text, world_size=None, start_rank=0):
         from ..models.layers_extra import convert_splitbn_model
 
         model = convert_splitbn_model(model, max(num_aug_splits, 2))
+
+    if args.group_norm:
+        assert not (args.split_bn or args.sync_bn), \
+            "--group-norm leaves no BatchNorm to split or to synchronize"
+        from ..models.layers_extra import convert_groupnorm_model
+
+        model = convert_groupnorm_model(model, args.group_norm)
 
     model = model.to(device)
     if use_cuda:
