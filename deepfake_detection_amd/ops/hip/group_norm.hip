@@ -40,7 +40,9 @@ GnPlan gn_plan(const GnArgs& a) {
   for (const void* p : ptrs)
     while (vec > 1 && !gn_aligned(p, vec * es)) vec >>= 1;
   const DfdPlan p = dfd_plan(a.c / vec, a.hw, a.n);
-  return {vec, p.cpb, p.ctiles, p.chunks, p.rows_per_chunk};
+  // rounding up the rows of a chunk can leave the last chunks without any
+  const int chunks = (int)((a.hw + p.rows_per_chunk - 1) / p.rows_per_chunk);
+  return {vec, p.cpb, p.ctiles, chunks, p.rows_per_chunk};
 }
 
 // (count, mean, sum of squares about the mean) of a set of values; joining

@@ -28,6 +28,7 @@ SHAPES = [
     (40, 64, 32, 3, 5),    # many images
     (2, 1, 1, 8, 9),
     (7, 56, 8, 37, 41),
+    (1, 256, 4, 90, 91),   # fp32: fewer chunks of rows than were asked for
 ]
 
 
