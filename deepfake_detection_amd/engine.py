@@ -61,7 +61,9 @@ def _use_fused_head(model, loss_fn, target, use_cuda) -> bool:
 
 def train_epoch(epoch, model, loader, optimizer, loss_fn, args, device,
                 lr_scheduler=None, saver=None, output_dir="", model_ema=None,
-                world_size=1, rank=0, num_epochs=None):
+                world_size=1, rank=0, num_epochs=None, teacher=None):
+    """One epoch. With a teacher (a model in eval mode), loss_fn takes its
+    output for the same input as a third argument (loss.TopKDistillLoss)."""
     use_cuda = device.type == "cuda"
     use_amp = bool(getattr(args, "amp", False)) and use_cuda
 
@@ -103,7 +105,12 @@ def train_epoch(epoch, model, loader, optimizer, loss_fn, args, device,
         else:
             with _autocast(use_amp):
                 output = model(input)
-                loss = loss_fn(output, target)
+                if teacher is None:
+                    loss = loss_fn(output, target)
+                else:
+                    with torch.no_grad():
+                        teacher_output = teacher(input)
+                    loss = loss_fn(output, target, teacher_output)
 
         optimizer.zero_grad(set_to_none=True)
         loss.backward()

@@ -163,6 +163,96 @@ def group_norm_act(x, gn, act: str = "silu", residual=None, drop_path_mask=None)
         x, gn.num_groups, gn.weight, gn.bias, gn.eps, act, residual, drop_path_mask)
 
 
+_LOGIT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MAX_TOPK = 256
+_MAX_DISTILL_CLASSES = 1 << 18
+
+
+def _check_logits(op, logits, k, temperature):
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"{op}: [..., classes] expected, got {tuple(logits.shape)}")
+    if logits.is_cuda and logits.dtype not in _LOGIT_DTYPES:
+        raise TypeError(f"{op}: float32, bfloat16 or float16 expected, got {logits.dtype}")
+    if not logits.is_floating_point():
+        raise TypeError(f"{op}: floating-point logits expected, got {logits.dtype}")
+    if not 1 <= k <= _MAX_TOPK:
+        raise ValueError(f"{op}: k must be in 1..{_MAX_TOPK}, got {k}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{op}: temperature must be in 1e-6..1e6, got {temperature}")
+
+
+def topk_logits(logits, k: int, temperature: float = 1.0):
+    """A teacher's answer, short: the k largest logits of each row and what is
+    left of it. Returns (values, indices, rest):
+
+      values   [..., k]  the logits themselves, largest first, in logits' type
+      indices  [..., k]  int64, their classes; equal logits by lowest class; -1
+                         where the logit is -inf (a class that is switched off)
+      rest     [...]     fp32, log(sum(exp(logit / temperature))) over the
+                         classes that were not taken; -inf if none is left
+
+    NaN counts as the largest value. logits: [..., classes], any row spacing;
+    1 <= k <= 256 and no more than classes. No gradient: what a teacher says is
+    given. GPU: one pass over the logits (ops/hip/distill.hip).
+    """
+    _check_logits("topk_logits", logits, k, temperature)
+    if k > logits.shape[-1]:
+        raise ValueError(f"topk_logits: k is {k}, of {logits.shape[-1]} classes")
+    if logits.is_cuda and gpu_ops_required():
+        return tuple(load_extension().topk_logits(logits, k, temperature))
+    return reference.topk_logits_forward(logits, k, temperature)
+
+
+def distill_topk(logits, values, indices, rest=None, temperature: float = 1.0):
+    """Loss of a student's logits against a teacher's top logits, one fp32
+    value for each row: the divergence KL(teacher || student) at the given
+    temperature over the classes that the teacher names and, as one class more,
+    all others together.
+
+      logits   [..., classes] of the student, any row spacing, at most 2^18
+               classes; fp32, bf16 or fp16; the gradient comes in their type
+      values, indices, rest   as topk_logits gives them, at the same
+               temperature; values of any of the three types, at most 256 slots.
+               Without rest the teacher's answer is its named classes alone.
+
+    A slot whose index is negative is empty. A row of empty slots without a
+    finite rest teaches nothing: its loss and gradient are 0, whatever its
+    logits hold. An index beyond the classes makes its row's loss and gradient
+    NaN. If two slots name one class, each has its own term in the loss and their
+    probabilities add up in the gradient. A class at -inf has student probability 0; where the teacher gives it more, the loss
+    is inf. The loss is not scaled by temperature^2. Differentiable once, in
+    logits; the teacher's answer is given. GPU: one pass over the logits
+    forward, one backward (ops/hip/distill.hip).
+    """
+    k = values.shape[-1] if values.dim() else 0
+    _check_logits("distill_topk", logits, k, temperature)
+    if logits.shape[-1] > _MAX_DISTILL_CLASSES:
+        raise ValueError(f"distill_topk: at most {_MAX_DISTILL_CLASSES} classes, "
+                         f"got {logits.shape[-1]}")
+    if values.shape[:-1] != logits.shape[:-1]:
+        raise ValueError(f"distill_topk: values must be [{logits.shape[:-1]}, k], "
+                         f"got {tuple(values.shape)}")
+    if indices.shape != values.shape:
+        raise ValueError(f"distill_topk: indices must be {tuple(values.shape)}, "
+                         f"got {tuple(indices.shape)}")
+    if indices.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"distill_topk: int64 or int32 indices expected, got {indices.dtype}")
+    if rest is not None and rest.shape != logits.shape[:-1]:
+        raise ValueError(f"distill_topk: rest must be {tuple(logits.shape[:-1])}, "
+                         f"got {tuple(rest.shape)}")
+    for name, t in (("values", values), ("rest", rest)):
+        if t is None:
+            continue
+        if t.requires_grad:
+            raise ValueError(f"distill_topk: {name} has no gradient: detach it")
+        if not t.is_floating_point() or (t.is_cuda and t.dtype not in _LOGIT_DTYPES):
+            raise TypeError(f"distill_topk: {name} must be float32, bfloat16 or float16, "
+                            f"got {t.dtype}")
+    if logits.is_cuda and gpu_ops_required():
+        return load_extension().distill_topk(logits, values, indices, rest, temperature)
+    return reference.distill_topk_forward(logits, values, indices, rest, temperature)
+
+
 def se(x, conv_reduce, act_module, conv_expand):
     """Squeeze-excite chain (pool -> 1x1 -> act -> 1x1 -> sigmoid -> mul).
 

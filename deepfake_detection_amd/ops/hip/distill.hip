@@ -1,0 +1,615 @@
+// A teacher's k largest logits, and the loss of a student against them with
+// its gradient, gfx950.
+//
+// topk: the k largest of a row, largest first, equal ones by lowest index,
+// and rest = log sum exp(t_i / T) over the classes that were not taken.
+//
+// distill: with u_j = v_j / T of the slots that name a class, the teacher's
+// answer is q = softmax over (u_1 .. u_k, rest): one probability for each
+// named class and one, q_r, for all others together. The student's is
+// p = softmax(z / T), p_r its sum over the classes that no slot names.
+//
+//   loss = sum_j q_j log(q_j / p_{i_j}) + q_r log(q_r / p_r)
+//   dz_i = (g / T) (p_i - sum of the q_j that name i)     i named
+//   dz_i = (g / T) p_i (1 - q_r / p_r)                    the rest
+//
+// The rest has a maximum and a sum of its own: as 1 - (what is named) it
+// would lose all its digits where a few classes hold nearly everything. The
+// loss is summed as q log(q / p) - q + p, whose terms do not cancel where the
+// two answers are near to each other; q and p both sum to one, so the sum is
+// the same.
+//
+// One block takes a row. All sums are made in a fixed order: the same inputs
+// give the same bits.
+
+#include "common.h"
+#include "distill.h"
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;
+
+// Sum of exp2((z - m) c) over a set of z, with the set's largest for m. An
+// empty set, or one of -inf alone, is {kLowest, 0}.
+struct Sum {
+  float m, s;
+};
+
+// One instruction; results below 2^-126 are 0.
+DFD_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+DFD_DEV void add(Sum& a, float z, float c) {
+  if (z > a.m) {
+    a.s = a.s * exp2_fast((a.m - z) * c) + 1.f;
+    a.m = z;
+  } else {
+    // equal: also where both are +inf, whose difference is no number
+    a.s += z == a.m ? 1.f : exp2_fast((z - a.m) * c);
+  }
+}
+
+DFD_DEV Sum join(const Sum& a, const Sum& b, float c) {
+  if (a.m == b.m) return {a.m, a.s + b.s};
+  return a.m > b.m ? Sum{a.m, a.s + b.s * exp2_fast((b.m - a.m) * c)}
+                   : Sum{b.m, b.s + a.s * exp2_fast((a.m - b.m) * c)};
+}
+
+DFD_DEV Sum wave_join(Sum v, float c) {
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) {
+    const Sum o = {__shfl_xor(v.m, off), __shfl_xor(v.s, off)};
+    v = lane & off ? join(o, v, c) : join(v, o, c);
+  }
+  return v;
+}
+
+// Every thread gets the block's sum.
+template <int THREADS>
+DFD_DEV Sum block_join(Sum v, float c, Sum* lds) {
+  v = wave_join(v, c);
+  if (THREADS == kWave) return v;
+  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
+  __syncthreads();
+  v = lds[0];
+  for (int w = 1; w < THREADS / kWave; ++w) v = join(v, lds[w], c);
+  return v;
+}
+
+// A row as aligned vectors: head elements before the first one, body vectors,
+// tail elements after the last.
+template <typename T, int VEC>
+struct Row {
+  const T* p;
+  int head, body, tail;
+  DFD_DEV Row(const T* row, int n) : p(row) {
+    const unsigned off = (unsigned)(reinterpret_cast<unsigned long long>(row) % (VEC * sizeof(T)));
+    head = off ? (int)((VEC * sizeof(T) - off) / sizeof(T)) : 0;
+    if (head > n) head = n;
+    body = (n - head) / VEC;
+    tail = n - head - body * VEC;
+  }
+  DFD_DEV DfdVec<T, VEC> load(int v) const { return dfd_vload<T, VEC>(p + head + (long long)v * VEC); }
+  DFD_DEV int first(int v) const { return head + v * VEC; }
+  DFD_DEV int edges() const { return head + tail; }
+  DFD_DEV int edge(int e) const { return e < head ? e : head + body * VEC + (e - head); }
+  DFD_DEV float at(int i) const { return DfdCvt<T>::to_f32(p[i]); }
+};
+
+// Order-preserving keys: any NaN is the largest, -0 and 0 are equal, and 0 is
+// below every value's key.
+DFD_DEV unsigned key_of(float f) {
+  if (f != f) return 0xffffffffu;
+  const unsigned u = f == 0.f ? 0u : __float_as_uint(f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// The leading bits of a key that can differ from the rest of it.
+template <typename T> constexpr int key_bits() { return 32; }
+template <> constexpr int key_bits<__hip_bfloat16>() { return 16; }
+template <> constexpr int key_bits<__half>() { return 19; }
+
+template <int THREADS>
+DFD_DEV int block_count(bool yes) {
+  if (THREADS == kWave) return __popcll(__ballot(yes));
+  return __syncthreads_count(yes);
+}
+
+// The place of each thread that says yes among them, in thread order.
+template <int THREADS>
+DFD_DEV int block_rank(bool yes, int* lds, int& total) {
+  const unsigned long long mask = __ballot(yes);
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wid = threadIdx.x / kWave;
+  int rank = __popcll(mask & ((1ull << lane) - 1));
+  if (THREADS == kWave) {
+    total = __popcll(mask);
+    return rank;
+  }
+  __syncthreads();  // lds may still be read
+  if (lane == 0) lds[wid] = __popcll(mask);
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < THREADS / kWave; ++w) {
+    if (w == wid) rank += total;
+    total += lds[w];
+  }
+  return rank;
+}
+
+// ---------------------------------------------------------------------------
+// topk
+// ---------------------------------------------------------------------------
+//
+// One pass over the row gives every thread the largest key and the sum of its
+// own elements. The k-th largest of the threads' largest is at most the row's
+// k-th largest: what lies below that bound is not taken. Only the threads
+// whose largest reaches it (about k of them) hold candidates; their elements
+// are read again, from the cache, by all threads together, and sorted into
+// candidates and rest. A candidate's rank is the number of greater ones.
+//
+// Many values equal to the bound can leave more candidates than fit; then the
+// k-th key is found by bisection over the whole row (topk_wide).
+
+template <int THREADS>
+constexpr int topk_cap() {
+  return THREADS == 64 ? 512 : THREADS == 256 ? 1024 : 2048;
+}
+
+template <int THREADS>
+struct TopkLds {
+  unsigned long long cand[topk_cap<THREADS>()];
+  float left[topk_cap<THREADS>()];  // candidates that were not taken, by rank
+  unsigned short hot[THREADS];
+  Sum sums[THREADS / kWave];
+  int counts[THREADS / kWave];
+  int n;
+};
+
+// The largest prefix that at least k of the threads' keys reach.
+template <int THREADS, int BITS>
+DFD_DEV unsigned topk_bound(unsigned key, int k) {
+  unsigned bound = 0;
+  for (int b = 31; b > 31 - BITS; --b) {
+    const unsigned test = bound | (1u << b);
+    const int n = block_count<THREADS>(key >= test);
+    if (n >= k) bound = test;
+    if (n == k) break;
+  }
+  return bound;
+}
+
+// Fills lds.cand with exactly the k to take; returns the sum of this thread's
+// share of the others.
+template <typename T, int THREADS>
+DFD_DEV Sum topk_wide(const T* row, int classes, int k, float c, TopkLds<THREADS>& lds) {
+  const int tid = threadIdx.x;
+  unsigned kth = 0;  // the k-th largest key
+  for (int b = 31; b >= 0; --b) {
+    const unsigned test = kth | (1u << b);
+    int mine = 0;
+    for (int i = tid; i < classes; i += THREADS) mine += key_of(DfdCvt<T>::to_f32(row[i])) >= test;
+    __syncthreads();
+    if (tid == 0) lds.n = 0;
+    __syncthreads();
+    atomicAdd(&lds.n, mine);
+    __syncthreads();
+    if (lds.n >= k) kth = test;
+  }
+  __syncthreads();
+  if (tid == 0) lds.n = 0;
+  __syncthreads();
+  for (int i = tid; i < classes; i += THREADS) {
+    const unsigned key = key_of(DfdCvt<T>::to_f32(row[i]));
+    if (key > kth) {  // fewer than k of them
+      const int at = atomicAdd(&lds.n, 1);
+      lds.cand[at] = ((unsigned long long)key << 32) | (unsigned)~i;
+    }
+  }
+  __syncthreads();
+  int have = lds.n;
+  int last = -1;  // the highest index taken of those equal to kth
+  for (int base = 0; have < k; base += THREADS) {
+    const int i = base + tid;
+    const bool equal = i < classes && key_of(DfdCvt<T>::to_f32(row[i])) == kth;
+    int total;
+    const int at = have + block_rank<THREADS>(equal, lds.counts, total);
+    if (equal && at < k) lds.cand[at] = ((unsigned long long)kth << 32) | (unsigned)~i;
+    have += total;
+    last = base + THREADS - 1;
+  }
+  __syncthreads();
+  if (tid == 0) lds.n = k;
+  // of the last tile some may be left over: those after the last one taken
+  unsigned lowest = 0xffffffffu;
+  for (int i = tid; i < k; i += THREADS)
+    if ((unsigned)(lds.cand[i] >> 32) == kth) {
+      const unsigned inv = (unsigned)lds.cand[i];
+      lowest = inv < lowest ? inv : lowest;
+    }
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) {
+    const unsigned o = __shfl_xor(lowest, off);
+    lowest = o < lowest ? o : lowest;
+  }
+  __syncthreads();
+  if ((tid & (kWave - 1)) == 0) lds.counts[tid / kWave] = (int)lowest;
+  __syncthreads();
+  for (int w = 0; w < THREADS / kWave; ++w)
+    lowest = (unsigned)lds.counts[w] < lowest ? (unsigned)lds.counts[w] : lowest;
+  last = (int)~lowest;
+  Sum mine = {kLowest, 0.f};
+  for (int i = tid; i < classes; i += THREADS) {
+    const float z = DfdCvt<T>::to_f32(row[i]);
+    const unsigned key = key_of(z);
+    if (key < kth || (key == kth && i > last)) add(mine, z, c);
+  }
+  return mine;
+}
+
+template <typename T, int VEC, int THREADS>
+__global__ __launch_bounds__(THREADS) void topk_kernel(
+    const T* __restrict__ logits, long long row_stride, int classes, int k, float inv_t,
+    T* __restrict__ values, long long* __restrict__ indices, float* __restrict__ rest) {
+  __shared__ TopkLds<THREADS> lds;
+  constexpr int kCap = topk_cap<THREADS>();
+  constexpr int kBits = key_bits<T>();
+  const int tid = threadIdx.x;
+  const long long r = blockIdx.x;
+  const T* p = logits + r * row_stride;
+  const Row<T, VEC> row(p, classes);
+  const float c = inv_t * kLog2e;
+
+  Sum mine = {kLowest, 0.f};
+  for (int v = tid; v < row.body; v += THREADS) {
+    const DfdVec<T, VEC> x = row.load(v);
+    float z[VEC], top = kLowest;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      z[i] = DfdCvt<T>::to_f32(x.v[i]);
+      top = fmaxf(top, z[i]);
+    }
+    if (top > mine.m) {
+      mine.s *= exp2_fast((mine.m - top) * c);
+      mine.m = top;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) mine.s += exp2_fast((z[i] - mine.m) * c);
+  }
+  unsigned key = 0;
+  if (tid < row.body) {
+    key = mine.s == 0.f ? key_of(-__builtin_inff()) : key_of(mine.m);
+    if (mine.s != mine.s) {  // a NaN or +inf among them
+      key = 0;
+      for (int v = tid; v < row.body; v += THREADS)
+        for (int i = 0; i < VEC; ++i) {
+          const unsigned o = key_of(row.at(row.first(v) + i));
+          key = o > key ? o : key;
+        }
+    }
+  }
+  if (tid == 0) lds.n = 0;
+  const unsigned bound = topk_bound<THREADS, kBits>(key, k);
+
+  const bool hot = tid < row.body && (key >= bound || mine.s != mine.s);
+  int nhot;
+  const int place = block_rank<THREADS>(hot, lds.counts, nhot);
+  if (hot) {
+    lds.hot[place] = (unsigned short)tid;
+    mine = {kLowest, 0.f};
+  }
+  __syncthreads();
+  auto sift = [&](float z, int i) {
+    const unsigned o = key_of(z);
+    if (o >= bound) {
+      const int at = atomicAdd(&lds.n, 1);
+      if (at < kCap) lds.cand[at] = ((unsigned long long)o << 32) | (unsigned)~i;
+    } else {
+      add(mine, z, c);
+    }
+  };
+  const int per = (row.body + THREADS - 1) / THREADS;
+  for (int w = tid; w < nhot * per; w += THREADS) {
+    const int j = w / nhot;
+    const int v = j * THREADS + lds.hot[w - j * nhot];
+    if (v < row.body) {
+      const DfdVec<T, VEC> x = row.load(v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sift(DfdCvt<T>::to_f32(x.v[i]), row.first(v) + i);
+    }
+  }
+  for (int e = tid; e < row.edges(); e += THREADS) sift(row.at(row.edge(e)), row.edge(e));
+  __syncthreads();
+  if (lds.n > kCap) {
+    mine = topk_wide<T, THREADS>(p, classes, k, c, lds);
+    __syncthreads();
+  }
+  const int n = lds.n;
+  for (int i = tid; i < n; i += THREADS) {
+    const unsigned long long own = lds.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += lds.cand[j] > own;
+    const int at = (int)~(unsigned)own;
+    if (rank < k) {
+      const T x = p[at];
+      values[r * k + rank] = x;
+      indices[r * k + rank] = DfdCvt<T>::to_f32(x) == -__builtin_inff() ? -1 : at;
+    } else {
+      lds.left[rank - k] = row.at(at);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n - k; i += THREADS) add(mine, lds.left[i], c);
+  const Sum all = block_join<THREADS>(mine, c, lds.sums);
+  if (tid == 0) rest[r] = all.s == 0.f ? -__builtin_inff() : all.m * inv_t + logf(all.s);
+}
+
+// ---------------------------------------------------------------------------
+// distill
+// ---------------------------------------------------------------------------
+
+DFD_DEV float load_as(const void* p, LogitType type, long long i) {
+  switch (type) {
+    case LogitType::kBf16:
+      return DfdCvt<__hip_bfloat16>::to_f32(static_cast<const __hip_bfloat16*>(p)[i]);
+    case LogitType::kF16: return DfdCvt<__half>::to_f32(static_cast<const __half*>(p)[i]);
+    default: return static_cast<const float*>(p)[i];
+  }
+}
+
+// What the backward pass needs of a row.
+struct RowStats {
+  float m_rest, coef;   // rest: dz = (g / T) coef exp2((z - m_rest) c)
+  float m, inv_s;       // named: p = exp2((z - m) c) inv_s
+  float u_top, inv_q;   // q_j = exp(u_j - u_top) inv_q
+  float state, unused;
+};
+static_assert(sizeof(RowStats) == kDistillStats * sizeof(float), "stats");
+
+constexpr float kTeaches = 0.f, kTwice = 1.f, kNothing = 2.f, kBadIndex = 3.f;
+
+template <typename T, int VEC, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_fwd_kernel(
+    const T* __restrict__ logits, long long row_stride, int classes, int k, float inv_t,
+    const void* __restrict__ values, LogitType vtype, const long long* __restrict__ indices,
+    const float* __restrict__ rest, float* __restrict__ loss, RowStats* __restrict__ stats) {
+  extern __shared__ unsigned bits[];  // one for each class: named by a slot
+  __shared__ int s_index[kMaxTopK];
+  __shared__ float s_u[kMaxTopK], s_z[kMaxTopK];
+  __shared__ unsigned char s_first[kMaxTopK];  // the first slot that names its class
+  __shared__ Sum sums[THREADS / kWave];
+  __shared__ int twice, bad;
+  const int tid = threadIdx.x;
+  const long long r = blockIdx.x;
+  const Row<T, VEC> row(logits + r * row_stride, classes);
+  const float c = inv_t * kLog2e;
+  // a vector's bits begin at a multiple of VEC
+  const int pad = row.head ? VEC - row.head : 0;
+  const int words = (classes + pad + 31) / 32;
+  for (int i = tid; i < words; i += THREADS) bits[i] = 0;
+  if (tid == 0) twice = bad = 0;
+  __syncthreads();
+  for (int j = tid; j < k; j += THREADS) {
+    const long long at = indices[r * k + j];
+    const bool in = at >= 0 && at < classes;
+    s_index[j] = in ? (int)at : -1;
+    s_u[j] = in ? load_as(values, vtype, r * k + j) * inv_t : -__builtin_inff();
+    s_z[j] = in ? row.at((int)at) : -__builtin_inff();
+    s_first[j] = 1;
+    if (at >= classes) bad = 1;
+    if (in) {
+      const unsigned b = (unsigned)at + pad;
+      if (atomicOr(&bits[b / 32], 1u << (b % 32)) >> (b % 32) & 1) twice = 1;
+    }
+  }
+  __syncthreads();
+  if (twice)
+    for (int j = tid; j < k; j += THREADS)
+      for (int i = 0; i < j; ++i)
+        if (s_index[i] == s_index[j]) s_first[j] = 0;
+
+  Sum mine = {kLowest, 0.f};
+  const unsigned char* marks = reinterpret_cast<const unsigned char*>(bits);
+  for (int v = tid; v < row.body; v += THREADS) {
+    const DfdVec<T, VEC> x = row.load(v);
+    const int b = row.first(v) + pad;
+    const unsigned mark = (marks[b / 8] >> (b % 8)) & ((1u << VEC) - 1);
+    float z[VEC], top = kLowest;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      z[i] = DfdCvt<T>::to_f32(x.v[i]);
+      if (mark >> i & 1) z[i] = -__builtin_inff();
+      top = fmaxf(top, z[i]);
+    }
+    if (top > mine.m) {
+      mine.s *= exp2_fast((mine.m - top) * c);
+      mine.m = top;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) mine.s += exp2_fast((z[i] - mine.m) * c);
+  }
+  for (int e = tid; e < row.edges(); e += THREADS) {
+    const int b = row.edge(e) + pad;
+    if (!(marks[b / 8] >> (b % 8) & 1)) add(mine, row.at(row.edge(e)), c);
+  }
+  const Sum others = block_join<THREADS>(mine, c, sums);
+  __syncthreads();  // s_first
+  if (tid >= kWave) return;
+
+  // the first wave: the row's few named classes
+  const float inf = __builtin_inff();
+  const float u_rest = rest ? rest[r] : -inf;
+  Sum named = {kLowest, 0.f};
+  float u_top = u_rest;
+  bool none = u_rest == u_rest;  // no NaN among the teacher's logits
+  for (int j = tid; j < k; j += kWave) {
+    u_top = fmaxf(u_top, s_u[j]);
+    none &= s_u[j] == s_u[j];
+    if (s_index[j] >= 0 && s_first[j]) add(named, s_z[j], c);
+  }
+  named = wave_join(named, c);
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) u_top = fmaxf(u_top, __shfl_xor(u_top, off));
+  const bool nothing = u_top == -inf && __all(none);
+  float q_sum = tid == 0 ? expf(u_rest - u_top) : 0.f;
+  for (int j = tid; j < k; j += kWave)
+    if (s_index[j] >= 0) q_sum += expf(s_u[j] - u_top);
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) q_sum += __shfl_xor(q_sum, off);
+  const Sum all = join(others, named, c);
+  const float log_q = logf(q_sum), log_s = logf(all.s);
+  float sum = 0.f;
+  auto term = [&](float lq, float lp) {
+    const float q = expf(lq);
+    if (q > 0.f) sum += q * (lq - lp) + (twice ? 0.f : expf(lp) - q);
+    else if (!twice) sum += expf(lp);
+  };
+  for (int j = tid; j < k; j += kWave)
+    if (s_index[j] >= 0) term(s_u[j] - u_top - log_q, (s_z[j] - all.m) * inv_t - log_s);
+  float p_rest = 0.f;
+  const float q_rest = expf(u_rest - u_top - log_q);
+  if (others.s != 0.f) {
+    const float lp = (others.m - all.m) * inv_t + logf(others.s) - log_s;
+    p_rest = expf(lp);
+    if (tid == 0) term(u_rest - u_top - log_q, lp);
+  } else if (tid == 0 && q_rest > 0.f) {
+    sum = inf;  // the teacher sees classes that the student rules out
+  }
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+  if (tid == 0) {
+    loss[r] = bad ? __builtin_nanf("") : nothing ? 0.f : sum;
+    RowStats s;
+    s.m_rest = others.m;
+    s.coef = others.s == 0.f ? 0.f : (p_rest - q_rest) / others.s;
+    s.m = all.m;
+    s.inv_s = 1.f / all.s;
+    s.u_top = u_top;
+    s.inv_q = 1.f / q_sum;
+    s.state = bad ? kBadIndex : nothing ? kNothing : twice ? kTwice : kTeaches;
+    s.unused = 0.f;
+    stats[r] = s;
+  }
+}
+
+template <typename T, int VEC, int THREADS>
+__global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
+    const T* __restrict__ logits, long long row_stride, int classes, int k, float inv_t,
+    const void* __restrict__ values, LogitType vtype, const long long* __restrict__ indices,
+    const RowStats* __restrict__ stats, const float* __restrict__ upstream,
+    long long upstream_stride, T* __restrict__ grad) {
+  const int tid = threadIdx.x;
+  const long long r = blockIdx.x;
+  const Row<T, VEC> row(logits + r * row_stride, classes);
+  const float c = inv_t * kLog2e;
+  T* out = grad + r * classes;
+  const RowStats s = stats[r];
+  const float g = upstream[r * upstream_stride] * inv_t;
+  if (s.state >= kNothing) {
+    const T fill = DfdCvt<T>::from_f32(s.state == kNothing ? 0.f : __builtin_nanf(""));
+    DfdVec<T, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = fill;
+    for (int v = tid; v < row.body; v += THREADS) dfd_vstore<T, VEC>(out + row.first(v), o);
+    for (int e = tid; e < row.edges(); e += THREADS) out[row.edge(e)] = fill;
+    return;
+  }
+  const float coef = s.coef * g;
+  for (int v = tid; v < row.body; v += THREADS) {
+    const DfdVec<T, VEC> x = row.load(v);
+    DfdVec<T, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      o.v[i] = DfdCvt<T>::from_f32(exp2_fast((DfdCvt<T>::to_f32(x.v[i]) - s.m_rest) * c) * coef);
+    dfd_vstore<T, VEC>(out + row.first(v), o);
+  }
+  for (int e = tid; e < row.edges(); e += THREADS) {
+    const int i = row.edge(e);
+    out[i] = DfdCvt<T>::from_f32(exp2_fast((row.at(i) - s.m_rest) * c) * coef);
+  }
+  // the named classes' gradients take the place of what was just written
+  __syncthreads();
+  for (int j = tid; j < k; j += THREADS) {
+    const long long at = indices[r * k + j];
+    if (at < 0) continue;
+    float q = 0.f;
+    if (s.state == kTwice) {
+      for (int i = 0; i < k; ++i)
+        if (indices[r * k + i] == at)
+          q += expf(load_as(values, vtype, r * k + i) * inv_t - s.u_top) * s.inv_q;
+    } else {
+      q = expf(load_as(values, vtype, r * k + j) * inv_t - s.u_top) * s.inv_q;
+    }
+    // (the exponential that keeps results below 2^-126)
+    const float p = expf((row.at((int)at) - s.m) * inv_t) * s.inv_s;
+    out[at] = DfdCvt<T>::from_f32((p - q) * g);
+  }
+}
+
+#define LOGIT_TYPE(VAL, ...)                                                 \
+  switch (VAL) {                                                             \
+    case LogitType::kF32: { using T = float; __VA_ARGS__; break; }           \
+    case LogitType::kBf16: { using T = __hip_bfloat16; __VA_ARGS__; break; } \
+    case LogitType::kF16: { using T = __half; __VA_ARGS__; break; }          \
+  }
+#define ROW_THREADS(VAL, ...)                                    \
+  switch (VAL) {                                                 \
+    case 64: { constexpr int N = 64; __VA_ARGS__; break; }       \
+    case 256: { constexpr int N = 256; __VA_ARGS__; break; }     \
+    default: { constexpr int N = 1024; __VA_ARGS__; break; }     \
+  }
+
+}  // namespace
+
+hipError_t topk_logits_launch(const TopkArgs& a, hipStream_t stream) {
+  const int threads = a.classes <= 4096 && a.k <= 32 ? 64 : a.classes <= 16384 && a.k <= 128 ? 256 : 1024;
+  const float inv_t = 1.f / a.temperature;
+  LOGIT_TYPE(a.type, ROW_THREADS(threads, {
+               constexpr int V = 16 / sizeof(T);
+               topk_kernel<T, V, N><<<dim3((unsigned)a.rows), N, 0, stream>>>(
+                   static_cast<const T*>(a.logits), a.row_stride, a.classes, a.k, inv_t,
+                   static_cast<T*>(a.values), a.indices, a.rest);
+             }));
+  return hipGetLastError();
+}
+
+hipError_t distill_fwd(const DistillArgs& a, hipStream_t stream) {
+  const int threads = a.classes <= 2048 ? 64 : a.classes <= 16384 ? 256 : 1024;
+  const float inv_t = 1.f / a.temperature;
+  const int bytes = (a.classes + 16 + 31) / 32 * 4;
+  LOGIT_TYPE(a.type, ROW_THREADS(threads, {
+               constexpr int V = 16 / sizeof(T);
+               distill_fwd_kernel<T, V, N><<<dim3((unsigned)a.rows), N, bytes, stream>>>(
+                   static_cast<const T*>(a.logits), a.row_stride, a.classes, a.k, inv_t,
+                   a.values, a.vtype, a.indices, a.rest, a.loss,
+                   reinterpret_cast<RowStats*>(a.stats));
+             }));
+  return hipGetLastError();
+}
+
+hipError_t distill_bwd(const DistillArgs& a, hipStream_t stream) {
+  const int threads = a.classes <= 2048 ? 64 : a.classes <= 16384 ? 256 : 1024;
+  const float inv_t = 1.f / a.temperature;
+  LOGIT_TYPE(a.type, ROW_THREADS(threads, {
+               constexpr int V = 16 / sizeof(T);
+               const T* z = static_cast<const T*>(a.logits);
+               T* grad = static_cast<T*>(a.grad);
+               // both rows' vectors lie alike, or elements go one by one
+               const bool alike =
+                   (reinterpret_cast<unsigned long long>(z) -
+                    reinterpret_cast<unsigned long long>(grad)) % 16 == 0 &&
+                   (a.row_stride - a.classes) * (long long)sizeof(T) % 16 == 0;
+               if (alike)
+                 distill_bwd_kernel<T, V, N><<<dim3((unsigned)a.rows), N, 0, stream>>>(
+                     z, a.row_stride, a.classes, a.k, inv_t, a.values, a.vtype, a.indices,
+                     reinterpret_cast<const RowStats*>(a.stats), a.upstream,
+                     a.upstream_stride, grad);
+               else
+                 distill_bwd_kernel<T, 1, N><<<dim3((unsigned)a.rows), N, 0, stream>>>(
+                     z, a.row_stride, a.classes, a.k, inv_t, a.values, a.vtype, a.indices,
+                     reinterpret_cast<const RowStats*>(a.stats), a.upstream,
+                     a.upstream_stride, grad);
+             }));
+  return hipGetLastError();
+}

@@ -58,6 +58,9 @@ at::Tensor group_norm_act(at::Tensor x, c10::optional<at::Tensor> weight,
                           c10::optional<at::Tensor> bias, int64_t groups, double eps,
                           std::string act, c10::optional<at::Tensor> residual,
                           c10::optional<at::Tensor> drop_path);
+std::vector<at::Tensor> topk_logits(at::Tensor logits, int64_t k, double temperature);
+at::Tensor distill_topk(at::Tensor logits, at::Tensor values, at::Tensor indices,
+                        c10::optional<at::Tensor> rest, double temperature);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "deepfake_detection_amd gfx950 (MI355X/CDNA4) kernels";
@@ -101,4 +104,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("groups"),
         py::arg("eps"), py::arg("act"), py::arg("residual") = py::none(),
         py::arg("drop_path") = py::none());
+  m.def("topk_logits", &topk_logits, "the k largest logits and the rest's log-sum-exp",
+        py::arg("logits"), py::arg("k"), py::arg("temperature"));
+  m.def("distill_topk", &distill_topk,
+        "loss against a teacher's top logits, differentiable in the student's",
+        py::arg("logits"), py::arg("values"), py::arg("indices"),
+        py::arg("rest") = py::none(), py::arg("temperature") = 1.0);
 }

@@ -1,5 +1,6 @@
-// Host side of the group norm + activation op: checks, allocation, autograd.
-// The kernels are in group_norm.hip.
+// Host side of the group norm + activation op and of the teacher's top logits
+// and their distillation: checks, allocation, autograd. The kernels are in
+// group_norm.hip and distill.hip.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -8,6 +9,7 @@
 #include <string>
 
 #include "common.h"
+#include "distill.h"
 #include "group_norm.h"
 
 namespace {
@@ -118,7 +120,135 @@ struct GroupNormAct : public torch::autograd::Function<GroupNormAct> {
   }
 };
 
+LogitType logit_type(const at::Tensor& x, const char* who) {
+  return static_cast<LogitType>(gn_type(x, who));
+}
+static_assert((int)LogitType::kBf16 == (int)GnType::kBf16 &&
+                  (int)LogitType::kF16 == (int)GnType::kF16,
+              "one numbering of types");
+
+// [..., classes] as [rows, classes] with unit stride in a row: a view where
+// the rows are evenly spaced, or else a copy.
+at::Tensor as_rows(const at::Tensor& x, const char* who) {
+  TORCH_CHECK(x.is_cuda() && x.dim() >= 1, who, ": CUDA logits expected");
+  const int64_t classes = x.size(-1);
+  TORCH_CHECK(classes >= 1 && classes <= INT_MAX - 64, who, ": ", classes, " classes");
+  auto rows = x.reshape({-1, classes});
+  TORCH_CHECK(rows.size(0) <= INT_MAX, who, ": too many rows");
+  return rows.stride(1) == 1 || classes == 1 ? rows : rows.contiguous();
+}
+
+struct DistillTopk : public torch::autograd::Function<DistillTopk> {
+  static at::Tensor forward(AutogradContext* ctx, at::Tensor logits, at::Tensor values,
+                            at::Tensor indices, OptTensor rest_opt, double temperature) {
+    const auto rest = rest_opt.value_or(at::Tensor());
+    const int64_t rows = logits.size(0);
+    auto opts = logits.options().dtype(at::kFloat);
+    auto loss = at::empty({rows}, opts);
+    auto stats = at::empty({rows, kDistillStats}, opts);
+    DistillArgs a = args(logits, values, indices, stats, temperature);
+    a.rest = f32_or_null(rest);
+    a.loss = loss.data_ptr<float>();
+    if (rows > 0)
+      check_launch(distill_fwd(a, at::hip::getCurrentHIPStream().stream()), "distill_topk");
+    ctx->save_for_backward({logits, values, indices, stats});
+    ctx->saved_data["temperature"] = temperature;
+    return loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "distill_topk: gradients of gradients are not supported");
+    auto saved = ctx->get_saved_variables();
+    const auto &logits = saved[0], &values = saved[1], &indices = saved[2], &stats = saved[3];
+    const c10::DeviceGuard guard(logits.device());
+    auto grad = at::empty(logits.sizes(), logits.options());
+    auto up = grads[0].to(at::kFloat);
+    DistillArgs a = args(logits, values, indices, stats, ctx->saved_data["temperature"].toDouble());
+    a.upstream = up.data_ptr<float>();
+    a.upstream_stride = up.stride(0);
+    a.grad = grad.data_ptr();
+    if (a.rows > 0)
+      check_launch(distill_bwd(a, at::hip::getCurrentHIPStream().stream()),
+                   "distill_topk backward");
+    return {grad, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+
+  static DistillArgs args(const at::Tensor& logits, const at::Tensor& values,
+                          const at::Tensor& indices, const at::Tensor& stats,
+                          double temperature) {
+    DistillArgs a = {};
+    a.logits = logits.data_ptr();
+    a.rows = logits.size(0);
+    a.row_stride = logits.stride(0);
+    a.classes = (int)logits.size(1);
+    a.k = (int)values.size(1);
+    a.type = logit_type(logits, "distill_topk");
+    a.vtype = logit_type(values, "distill_topk: values");
+    a.temperature = (float)temperature;
+    a.values = values.data_ptr();
+    a.indices = reinterpret_cast<const long long*>(indices.data_ptr<int64_t>());
+    a.stats = stats.data_ptr<float>();
+    return a;
+  }
+};
+
 }  // namespace
+
+std::vector<at::Tensor> topk_logits(at::Tensor logits, int64_t k, double temperature) {
+  const char* who = "topk_logits";
+  const LogitType type = logit_type(logits, who);
+  const c10::DeviceGuard guard(logits.device());
+  const at::Tensor x = as_rows(logits.detach(), who);
+  TORCH_CHECK(k >= 1 && k <= kMaxTopK && k <= x.size(1), who, ": k is ", k);
+  auto shape = logits.sizes().vec();
+  shape.back() = k;
+  auto values = at::empty(shape, logits.options());
+  auto indices = at::empty(shape, logits.options().dtype(at::kLong));
+  shape.pop_back();
+  auto rest = at::empty(shape, logits.options().dtype(at::kFloat));
+  TopkArgs a = {};
+  a.logits = x.data_ptr();
+  a.rows = x.size(0);
+  a.row_stride = x.stride(0);
+  a.classes = (int)x.size(1);
+  a.k = (int)k;
+  a.type = type;
+  a.temperature = (float)temperature;
+  a.values = values.data_ptr();
+  a.indices = reinterpret_cast<long long*>(indices.data_ptr<int64_t>());
+  a.rest = rest.data_ptr<float>();
+  if (a.rows > 0)
+    check_launch(topk_logits_launch(a, at::hip::getCurrentHIPStream().stream()), who);
+  return {values, indices, rest};
+}
+
+at::Tensor distill_topk(at::Tensor logits, at::Tensor values, at::Tensor indices,
+                        OptTensor rest_opt, double temperature) {
+  const char* who = "distill_topk";
+  logit_type(logits, who);
+  logit_type(values, "distill_topk: values");
+  const c10::DeviceGuard guard(logits.device());
+  const at::Tensor x = as_rows(logits, who);
+  const int64_t rows = x.size(0), k = values.size(-1);
+  TORCH_CHECK(x.size(1) <= kMaxDistillClasses, who, ": ", x.size(1), " classes");
+  TORCH_CHECK(k >= 1 && k <= kMaxTopK, who, ": k is ", k);
+  TORCH_CHECK(values.numel() == rows * k && indices.numel() == rows * k, who,
+              ": values and indices must be [rows, k]");
+  TORCH_CHECK(values.device() == x.device() && indices.device() == x.device(), who,
+              ": the teacher's answer must be on the device of the logits");
+  auto rest = rest_opt.has_value() && rest_opt->defined() ? *rest_opt : at::Tensor();
+  if (rest.defined()) {
+    TORCH_CHECK(rest.numel() == rows && rest.device() == x.device(), who,
+                ": rest must be [rows], on the device of the logits");
+    rest = rest.detach().to(at::kFloat).reshape({rows}).contiguous();
+  }
+  auto loss = DistillTopk::apply(
+      x, values.detach().reshape({rows, k}).contiguous(),
+      indices.to(at::kLong).reshape({rows, k}).contiguous(),
+      rest.defined() ? OptTensor(rest) : c10::nullopt, temperature);
+  return loss.reshape(logits.sizes().slice(0, logits.dim() - 1));
+}
 
 at::Tensor group_norm_act(at::Tensor x, OptTensor weight_opt,
                           OptTensor bias_opt, int64_t groups, double eps,

@@ -46,6 +46,50 @@ def group_norm_act_forward(x, num_groups, weight, bias, eps, act="silu", residua
     return y.to(x.dtype)
 
 
+def topk_logits_forward(logits, k, temperature=1.0):
+    """(values, indices, rest) of functional.topk_logits, by a stable sort."""
+    logits = logits.detach()
+    wide = torch.promote_types(logits.dtype, torch.float32)
+    values, indices = torch.sort(logits, dim=-1, descending=True, stable=True)
+    values, indices = values[..., :k].contiguous(), indices[..., :k].contiguous()
+    left = (logits.to(wide) / temperature).scatter(-1, indices, float("-inf"))
+    rest = torch.logsumexp(left, dim=-1)
+    return values, indices.masked_fill(values == float("-inf"), -1), rest.to(
+        torch.promote_types(torch.float32, rest.dtype))
+
+
+def distill_topk_forward(logits, values, indices, rest=None, temperature=1.0):
+    """The rows' losses of functional.distill_topk, in fp32 at least."""
+    wide = torch.promote_types(logits.dtype, torch.float32)
+    inf = float("inf")
+    shape, classes, k = logits.shape[:-1], logits.shape[-1], values.shape[-1]
+    z = logits.to(wide).reshape(-1, classes) / temperature
+    at = indices.reshape(-1, k).long()
+    slot = (at >= 0) & (at < classes)
+    bad = (at >= classes).any(dim=1)
+    at = torch.where(slot, at, 0)
+    u = (values.to(wide).reshape(-1, k) / temperature).masked_fill(~slot, -inf)
+    left = torch.full_like(z[:, 0].detach(), -inf) if rest is None else rest.to(wide).reshape(-1)
+    u = torch.cat([u, left[:, None]], dim=1)
+    teaches = (u != -inf).any(dim=1)
+    # what such a row holds must not reach its gradient either
+    z = torch.where((teaches | bad)[:, None], z, 0.0)
+    q = torch.softmax(torch.where(teaches[:, None], u, 0.0), dim=1)
+    named = torch.zeros(z.shape, device=z.device, dtype=wide)
+    named = named.scatter_add_(1, at, slot.to(wide)) > 0
+    # where the teacher leaves the rest nothing its sum has no part in the loss
+    counts = (q[:, -1:] > 0) & named & teaches[:, None]
+    log_rest = torch.logsumexp(z.masked_fill(counts, -inf), dim=1, keepdim=True)
+    log_p = torch.cat([z.gather(1, at), log_rest], dim=1) - torch.logsumexp(
+        z, dim=1, keepdim=True)
+    # q log q - q log p, with 0 for q = 0
+    loss = torch.where(q == 0, 0.0, torch.xlogy(q, q) - q * log_p).sum(dim=1)
+    loss = torch.where(teaches | bad, loss, 0.0)
+    # loss and gradient alike
+    loss = loss * torch.where(bad, float("nan"), 1.0)
+    return loss.reshape(shape)
+
+
 def se_forward(x, w_reduce, b_reduce, w_expand, b_expand, act="silu", gate="sigmoid"):
     """Squeeze-excite chain: global-avg-pool -> 1x1 reduce -> act -> 1x1
     expand -> sigmoid gate -> broadcast multiply

@@ -39,7 +39,7 @@ from ..data import (
     resolve_data_config,
 )
 from ..engine import train_epoch, validate
-from ..loss import LabelSmoothingCrossEntropy, SoftTargetCrossEntropy
+from ..loss import LabelSmoothingCrossEntropy, SoftTargetCrossEntropy, TopKDistillLoss
 from ..optim import create_optimizer
 from ..parallel import distribute_bn, init_distributed, parse_server, wrap_ddp
 from ..parallel.distributed import convert_sync_batchnorm
@@ -129,6 +129,17 @@ def _build_parser():
     parser.add_argument("--mixup-off-epoch", default=0, type=int)
     parser.add_argument("--smoothing", type=float, default=0.1)
     parser.add_argument("--train-interpolation", type=str, default="random")
+    # Distillation
+    parser.add_argument("--teacher", default="", type=str, metavar="MODEL",
+                        help="model whose answers the trained one learns from too")
+    parser.add_argument("--teacher-checkpoint", default="", type=str, metavar="PATH")
+    parser.add_argument("--teacher-group-norm", type=int, default=0, metavar="G",
+                        help="the teacher was trained with --group-norm G")
+    parser.add_argument("--distill-k", type=int, default=20, metavar="K",
+                        help="the teacher's K largest logits are learned")
+    parser.add_argument("--distill-temperature", type=float, default=2.0, metavar="T")
+    parser.add_argument("--distill-alpha", type=float, default=0.5, metavar="A",
+                        help="share of the teacher's part in the loss")
     # BatchNorm
     parser.add_argument("--bn-tf", action="store_true", default=False)
     parser.add_argument("--bn-momentum", type=float, default=None)
@@ -337,6 +348,23 @@ def main(rank, args, args_text, world_size=None, start_rank=0):
         train_loss_fn = torch.nn.CrossEntropyLoss().to(device)
     validate_loss_fn = torch.nn.CrossEntropyLoss().to(device)
 
+    teacher = None
+    if args.teacher:
+        assert not args.jsd, "--jsd's loss already compares the model with itself"
+        teacher = create_model(
+            args.teacher, num_classes=args.num_classes, in_chans=in_chans,
+            checkpoint_path=args.teacher_checkpoint)
+        if args.teacher_group_norm:
+            from ..models.layers_extra import convert_groupnorm_model
+
+            teacher = convert_groupnorm_model(teacher, args.teacher_group_norm)
+        teacher = teacher.to(device).eval().requires_grad_(False)
+        if use_cuda:
+            teacher = teacher.to(memory_format=torch.channels_last)
+        train_loss_fn = TopKDistillLoss(
+            train_loss_fn, k=args.distill_k, temperature=args.distill_temperature,
+            alpha=args.distill_alpha).to(device)
+
     eval_metric = args.eval_metric
     best_metric = None
     best_epoch = None
@@ -375,7 +403,8 @@ def main(rank, args, args_text, world_size=None, start_rank=0):
             train_metrics = train_epoch(
                 epoch, model, loader_train, optimizer, train_loss_fn, args, device,
                 lr_scheduler=lr_scheduler, saver=saver, output_dir=output_dir,
-                model_ema=model_ema, world_size=world_size, rank=whole_rank)
+                model_ema=model_ema, world_size=world_size, rank=whole_rank,
+                teacher=teacher)
 
             eval_metrics = validate(model, loader_eval, validate_loss_fn, args, device,
                                     world_size=world_size, rank=whole_rank)
