@@ -97,6 +97,74 @@ struct Row {
   DFD_DEV float at(int i) const { return DfdCvt<T>::to_f32(p[i]); }
 };
 
+// f(vector, its number) for the thread's vectors of a row. Four loads are in
+// flight at a time; those beyond the row load its last vector again and are
+// dropped, which costs less than a branch around each.
+template <int THREADS, typename T, int VEC, typename F>
+DFD_DEV void stream(const Row<T, VEC>& row, F f) {
+  constexpr int U = 4;
+  for (int v = threadIdx.x; v < row.body; v += U * THREADS) {
+    DfdVec<T, VEC> x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int w = v + u * THREADS;
+      x[u] = row.load(w < row.body ? w : row.body - 1);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v + u * THREADS < row.body) f(x[u], v + u * THREADS);
+  }
+}
+
+// The sum of a stream of vectors at one fma and one exponential a value:
+// exp2(z c - mc), mc = m c as it is rounded; what the rounding of mc shifted
+// all of them by is taken out at the end. Values at kDeep and below, as masks
+// of a type's lowest value are, count as 0; where they are all there is, the
+// caller sums again by add().
+constexpr float kDeep = -1e30f;
+
+struct FastSum {
+  float m, mc, s;
+  float seen;  // the largest value, also where that is below kDeep
+  DFD_DEV explicit FastSum(float c) : m(kDeep), mc(kDeep * c), s(0.f), seen(-__builtin_inff()) {}
+  template <int N>
+  DFD_DEV void add(const float (&z)[N], float c) {
+    float top = z[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, z[i]);
+    seen = fmaxf(seen, top);
+    if (top > m) {
+      m = top;
+      const float was = mc;
+      mc = top * c;
+      s *= exp2_fast(was - mc);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) s += exp2_fast(__builtin_fmaf(z[i], c, -mc));
+  }
+  DFD_DEV Sum get(float c) const {
+    if (s == 0.f) return {kLowest, 0.f};
+    return {m, s * exp2_fast(-__builtin_fmaf(m, c, -mc))};
+  }
+};
+
+template <typename T, int VEC>
+DFD_DEV void to_floats(const DfdVec<T, VEC>& x, float (&z)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) z[i] = DfdCvt<T>::to_f32(x.v[i]);
+}
+
+// A store of what this op does not read again.
+template <typename T, int VEC>
+DFD_DEV void store_once(T* p, const DfdVec<T, VEC>& x) {
+  if constexpr (VEC * sizeof(T) == 16) {
+    typedef unsigned Words __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(*reinterpret_cast<const Words*>(&x), reinterpret_cast<Words*>(p));
+  } else {
+    dfd_vstore<T, VEC>(p, x);
+  }
+}
+
 // Order-preserving keys: any NaN is the largest, -0 and 0 are equal, and 0 is
 // below every value's key.
 DFD_DEV unsigned key_of(float f) {
@@ -109,6 +177,8 @@ DFD_DEV unsigned key_of(float f) {
 template <typename T> constexpr int key_bits() { return 32; }
 template <> constexpr int key_bits<__hip_bfloat16>() { return 16; }
 template <> constexpr int key_bits<__half>() { return 19; }
+
+constexpr unsigned kOffKey = ~0xff800000u;  // the key of -inf
 
 template <int THREADS>
 DFD_DEV int block_count(bool yes) {
@@ -142,32 +212,36 @@ DFD_DEV int block_rank(bool yes, int* lds, int& total) {
 // topk
 // ---------------------------------------------------------------------------
 //
-// One pass over the row gives every thread the largest key and the sum of its
-// own elements. The k-th largest of the threads' largest is at most the row's
-// k-th largest: what lies below that bound is not taken. Only the threads
-// whose largest reaches it (about k of them) hold candidates; their elements
-// are read again, from the cache, by all threads together, and sorted into
-// candidates and rest. A candidate's rank is the number of greater ones.
+// One pass over the row: every thread takes its vectors in up to kParts parts
+// and keeps the largest value and the sum of each. The k-th largest of the
+// threads' largest is at most the row's k-th largest: what lies below that
+// bound is not taken. Only the parts whose largest reaches it (about k of
+// them) hold candidates; their elements are read again, from the cache, by all
+// threads together, and sorted into candidates and rest. A candidate's rank is
+// the number of greater ones. -inf is no candidate (nothing is said of a class
+// that is switched off), so a row may have fewer than k.
 //
 // Many values equal to the bound can leave more candidates than fit; then the
-// k-th key is found by bisection over the whole row (topk_wide).
+// row is searched as a whole (topk_wide).
+
+constexpr int kParts = 8;
 
 template <int THREADS>
 constexpr int topk_cap() {
-  return THREADS == 64 ? 512 : THREADS == 256 ? 1024 : 2048;
+  return THREADS == 64 ? 512 : 1024;
 }
 
 template <int THREADS>
 struct TopkLds {
   unsigned long long cand[topk_cap<THREADS>()];
   float left[topk_cap<THREADS>()];  // candidates that were not taken, by rank
-  unsigned short hot[THREADS];
+  unsigned short hot[THREADS * kParts];  // part * THREADS + thread
   Sum sums[THREADS / kWave];
   int counts[THREADS / kWave];
   int n;
 };
 
-// The largest prefix that at least k of the threads' keys reach.
+// The largest key that at least k of the threads' keys reach.
 template <int THREADS, int BITS>
 DFD_DEV unsigned topk_bound(unsigned key, int k) {
   unsigned bound = 0;
@@ -177,25 +251,40 @@ DFD_DEV unsigned topk_bound(unsigned key, int k) {
     if (n >= k) bound = test;
     if (n == k) break;
   }
-  return bound;
+  // the bits that a narrow type does not have are ones in a negative value's key
+  return bound >> 31 ? bound : bound | (unsigned)((1ull << (32 - BITS)) - 1);
+}
+
+template <int THREADS>
+DFD_DEV int block_total(int mine, int& lds) {
+  __syncthreads();
+  if (threadIdx.x == 0) lds = 0;
+  __syncthreads();
+  if (mine) atomicAdd(&lds, mine);
+  __syncthreads();
+  return lds;
 }
 
 // Fills lds.cand with exactly the k to take; returns the sum of this thread's
-// share of the others.
+// share of the others. At least k keys reach bound, which is no -inf.
 template <typename T, int THREADS>
-DFD_DEV Sum topk_wide(const T* row, int classes, int k, float c, TopkLds<THREADS>& lds) {
+DFD_DEV Sum topk_wide(const T* row, int classes, int k, float c, unsigned bound,
+                      TopkLds<THREADS>& lds) {
   const int tid = threadIdx.x;
-  unsigned kth = 0;  // the k-th largest key
-  for (int b = 31; b >= 0; --b) {
-    const unsigned test = kth | (1u << b);
+  auto above = [&](unsigned key) {
     int mine = 0;
-    for (int i = tid; i < classes; i += THREADS) mine += key_of(DfdCvt<T>::to_f32(row[i])) >= test;
-    __syncthreads();
-    if (tid == 0) lds.n = 0;
-    __syncthreads();
-    atomicAdd(&lds.n, mine);
-    __syncthreads();
-    if (lds.n >= k) kth = test;
+    for (int i = tid; i < classes; i += THREADS) mine += key_of(DfdCvt<T>::to_f32(row[i])) > key;
+    return block_total<THREADS>(mine, lds.n);
+  };
+  // the k-th largest key: the bound itself if values equal to it are what
+  // there are many of, or else by bisection
+  unsigned kth = bound;
+  if (above(bound) >= k) {
+    kth = 0;
+    for (int b = 31; b >= 0; --b) {
+      const unsigned test = kth | (1u << b);
+      if (above(test - 1) >= k) kth = test;
+    }
   }
   __syncthreads();
   if (tid == 0) lds.n = 0;
@@ -209,7 +298,6 @@ DFD_DEV Sum topk_wide(const T* row, int classes, int k, float c, TopkLds<THREADS
   }
   __syncthreads();
   int have = lds.n;
-  int last = -1;  // the highest index taken of those equal to kth
   for (int base = 0; have < k; base += THREADS) {
     const int i = base + tid;
     const bool equal = i < classes && key_of(DfdCvt<T>::to_f32(row[i])) == kth;
@@ -217,7 +305,6 @@ DFD_DEV Sum topk_wide(const T* row, int classes, int k, float c, TopkLds<THREADS
     const int at = have + block_rank<THREADS>(equal, lds.counts, total);
     if (equal && at < k) lds.cand[at] = ((unsigned long long)kth << 32) | (unsigned)~i;
     have += total;
-    last = base + THREADS - 1;
   }
   __syncthreads();
   if (tid == 0) lds.n = k;
@@ -238,7 +325,7 @@ DFD_DEV Sum topk_wide(const T* row, int classes, int k, float c, TopkLds<THREADS
   __syncthreads();
   for (int w = 0; w < THREADS / kWave; ++w)
     lowest = (unsigned)lds.counts[w] < lowest ? (unsigned)lds.counts[w] : lowest;
-  last = (int)~lowest;
+  const int last = (int)~lowest;  // the highest index taken of those equal to kth
   Sum mine = {kLowest, 0.f};
   for (int i = tid; i < classes; i += THREADS) {
     const float z = DfdCvt<T>::to_f32(row[i]);
@@ -261,58 +348,95 @@ __global__ __launch_bounds__(THREADS) void topk_kernel(
   const Row<T, VEC> row(p, classes);
   const float c = inv_t * kLog2e;
 
-  Sum mine = {kLowest, 0.f};
-  for (int v = tid; v < row.body; v += THREADS) {
-    const DfdVec<T, VEC> x = row.load(v);
-    float z[VEC], top = kLowest;
+  // part q: vectors from q * step on, `per` for each thread
+  constexpr int U = 4;
+  const int rounds = (row.body + U * kParts * THREADS - 1) / (U * kParts * THREADS);
+  const int per = U * (rounds > 0 ? rounds : 1);
+  const int step = per * THREADS;
+  Sum part[kParts];  // {largest value, sum}
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      z[i] = DfdCvt<T>::to_f32(x.v[i]);
-      top = fmaxf(top, z[i]);
-    }
-    if (top > mine.m) {
-      mine.s *= exp2_fast((mine.m - top) * c);
-      mine.m = top;
-    }
+  for (int q = 0; q < kParts; ++q) {
+    part[q] = {-__builtin_inff(), 0.f};
+    if (q * step >= row.body) continue;  // the same for the whole block
+    const int end = (q + 1) * step < row.body ? (q + 1) * step : row.body;
+    FastSum fast(c);
+    for (int v = q * step + tid; v < end; v += U * THREADS) {
+      DfdVec<T, VEC> x[U];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) mine.s += exp2_fast((z[i] - mine.m) * c);
+      for (int u = 0; u < U; ++u) {
+        const int w = v + u * THREADS;
+        x[u] = row.load(w < end ? w : end - 1);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v + u * THREADS < end) {
+          float z[VEC];
+          to_floats(x[u], z);
+          fast.add(z, c);
+        }
+    }
+    part[q] = {fast.seen, fast.get(c).s};
+    if (part[q].s != part[q].s || (part[q].s == 0.f && part[q].m > -__builtin_inff())) {
+      // a NaN or +inf among them, or values that FastSum does not count
+      part[q] = {-__builtin_inff(), 0.f};
+      for (int v = q * step + tid; v < end; v += THREADS)
+        for (int i = 0; i < VEC; ++i) add(part[q], row.at(row.first(v) + i), c);
+    }
   }
+  // a NaN leaves its mark in the sum alone
+  auto key_of_part = [&](int q) { return part[q].s != part[q].s ? 0xffffffffu : key_of(part[q].m); };
   unsigned key = 0;
   if (tid < row.body) {
-    key = mine.s == 0.f ? key_of(-__builtin_inff()) : key_of(mine.m);
-    if (mine.s != mine.s) {  // a NaN or +inf among them
-      key = 0;
-      for (int v = tid; v < row.body; v += THREADS)
-        for (int i = 0; i < VEC; ++i) {
-          const unsigned o = key_of(row.at(row.first(v) + i));
-          key = o > key ? o : key;
-        }
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+      const unsigned o = key_of_part(q);
+      key = o > key ? o : key;
     }
   }
   if (tid == 0) lds.n = 0;
   const unsigned bound = topk_bound<THREADS, kBits>(key, k);
 
-  const bool hot = tid < row.body && (key >= bound || mine.s != mine.s);
-  int nhot;
-  const int place = block_rank<THREADS>(hot, lds.counts, nhot);
-  if (hot) {
-    lds.hot[place] = (unsigned short)tid;
-    mine = {kLowest, 0.f};
+  // the hot parts' list, in a fixed order; the sum of the others
+  Sum mine = {kLowest, 0.f};
+  unsigned hot = 0;
+  int before = 0, count = 0;  // hot parts of lower lanes, and of the wave
+#pragma unroll
+  for (int q = 0; q < kParts; ++q) {
+    const unsigned o = key_of_part(q);
+    const bool is = o >= bound && o > kOffKey;
+    if (is) hot |= 1u << q;
+    else if (part[q].s > 0.f) mine = join(mine, part[q], c);
+    const unsigned long long all = __ballot(is);
+    before += __popcll(all & ((1ull << (tid & (kWave - 1))) - 1));
+    count += __popcll(all);
   }
+  int nhot = count;
+  if (THREADS > kWave) {
+    if ((tid & (kWave - 1)) == 0) lds.counts[tid / kWave] = count;
+    __syncthreads();
+    nhot = 0;
+    for (int w = 0; w < THREADS / kWave; ++w) {
+      if (w == tid / kWave) before += nhot;
+      nhot += lds.counts[w];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kParts; ++q)
+    if (hot >> q & 1) lds.hot[before++] = (unsigned short)(q * THREADS + tid);
   __syncthreads();
   auto sift = [&](float z, int i) {
     const unsigned o = key_of(z);
-    if (o >= bound) {
+    if (o >= bound && o > kOffKey) {
       const int at = atomicAdd(&lds.n, 1);
       if (at < kCap) lds.cand[at] = ((unsigned long long)o << 32) | (unsigned)~i;
     } else {
       add(mine, z, c);
     }
   };
-  const int per = (row.body + THREADS - 1) / THREADS;
   for (int w = tid; w < nhot * per; w += THREADS) {
-    const int j = w / nhot;
-    const int v = j * THREADS + lds.hot[w - j * nhot];
+    const int h = w / per;
+    const int q = lds.hot[h] / THREADS;
+    const int v = q * step + (w - h * per) * THREADS + lds.hot[h] % THREADS;
     if (v < row.body) {
       const DfdVec<T, VEC> x = row.load(v);
 #pragma unroll
@@ -322,7 +446,7 @@ __global__ __launch_bounds__(THREADS) void topk_kernel(
   for (int e = tid; e < row.edges(); e += THREADS) sift(row.at(row.edge(e)), row.edge(e));
   __syncthreads();
   if (lds.n > kCap) {
-    mine = topk_wide<T, THREADS>(p, classes, k, c, lds);
+    mine = topk_wide<T, THREADS>(p, classes, k, c, bound, lds);
     __syncthreads();
   }
   const int n = lds.n;
@@ -334,10 +458,14 @@ __global__ __launch_bounds__(THREADS) void topk_kernel(
     if (rank < k) {
       const T x = p[at];
       values[r * k + rank] = x;
-      indices[r * k + rank] = DfdCvt<T>::to_f32(x) == -__builtin_inff() ? -1 : at;
+      indices[r * k + rank] = at;
     } else {
       lds.left[rank - k] = row.at(at);
     }
+  }
+  for (int i = n + tid; i < k; i += THREADS) {
+    values[r * k + i] = DfdCvt<T>::from_f32(-__builtin_inff());
+    indices[r * k + i] = -1;
   }
   __syncthreads();
   for (int i = tid; i < n - k; i += THREADS) add(mine, lds.left[i], c);
@@ -409,32 +537,45 @@ __global__ __launch_bounds__(THREADS) void distill_fwd_kernel(
       for (int i = 0; i < j; ++i)
         if (s_index[i] == s_index[j]) s_first[j] = 0;
 
-  Sum mine = {kLowest, 0.f};
+  // Vectors without a named class are summed as they stream by; the others
+  // are left to the first slot that names a class of theirs.
   const unsigned char* marks = reinterpret_cast<const unsigned char*>(bits);
-  for (int v = tid; v < row.body; v += THREADS) {
-    const DfdVec<T, VEC> x = row.load(v);
+  constexpr unsigned kAll = (1u << VEC) - 1;
+  auto marks_of = [&](int v) {
     const int b = row.first(v) + pad;
-    const unsigned mark = (marks[b / 8] >> (b % 8)) & ((1u << VEC) - 1);
-    float z[VEC], top = kLowest;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      z[i] = DfdCvt<T>::to_f32(x.v[i]);
-      if (mark >> i & 1) z[i] = -__builtin_inff();
-      top = fmaxf(top, z[i]);
-    }
-    if (top > mine.m) {
-      mine.s *= exp2_fast((mine.m - top) * c);
-      mine.m = top;
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) mine.s += exp2_fast((z[i] - mine.m) * c);
-  }
-  for (int e = tid; e < row.edges(); e += THREADS) {
-    const int b = row.edge(e) + pad;
-    if (!(marks[b / 8] >> (b % 8) & 1)) add(mine, row.at(row.edge(e)), c);
-  }
-  const Sum others = block_join<THREADS>(mine, c, sums);
+    return (unsigned)(marks[b / 8] >> (b % 8)) & kAll;
+  };
+  auto named_at = [&](int i) { return marks[(i + pad) / 8] >> ((i + pad) % 8) & 1; };
+  FastSum fast(c);
+  stream<THREADS>(row, [&](const DfdVec<T, VEC>& x, int v) {
+    if (marks_of(v)) return;
+    float z[VEC];
+    to_floats(x, z);
+    fast.add(z, c);
+  });
+  Sum mine = fast.get(c);
+  for (int e = tid; e < row.edges(); e += THREADS)
+    if (!named_at(row.edge(e))) add(mine, row.at(row.edge(e)), c);
   __syncthreads();  // s_first
+  for (int j = tid; j < k; j += THREADS) {
+    const int i = s_index[j] - row.head;
+    if (i < 0 || i >= row.body * VEC || !s_first[j]) continue;
+    const int v = i / VEC;
+    const unsigned mark = marks_of(v);
+    if (mark & ((1u << (i % VEC)) - 1)) continue;
+    const DfdVec<T, VEC> x = row.load(v);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (!(mark >> e & 1)) add(mine, DfdCvt<T>::to_f32(x.v[e]), c);
+  }
+  Sum others = block_join<THREADS>(mine, c, sums);
+  if (others.m <= kDeep) {  // the same for the whole block
+    mine = {kLowest, 0.f};
+    for (int i = tid; i < classes; i += THREADS)
+      if (!named_at(i)) add(mine, row.at(i), c);
+    __syncthreads();
+    others = block_join<THREADS>(mine, c, sums);
+  }
   if (tid >= kWave) return;
 
   // the first wave: the row's few named classes
@@ -481,7 +622,7 @@ __global__ __launch_bounds__(THREADS) void distill_fwd_kernel(
   if (tid == 0) {
     loss[r] = bad ? __builtin_nanf("") : nothing ? 0.f : sum;
     RowStats s;
-    s.m_rest = others.m;
+    s.m_rest = others.s == 0.f ? 0.f : others.m;
     s.coef = others.s == 0.f ? 0.f : (p_rest - q_rest) / others.s;
     s.m = all.m;
     s.inv_s = 1.f / all.s;
@@ -500,7 +641,8 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
     const RowStats* __restrict__ stats, const float* __restrict__ upstream,
     long long upstream_stride, T* __restrict__ grad) {
   const int tid = threadIdx.x;
-  const long long r = blockIdx.x;
+  // from the last row on: what the forward pass read last may still be cached
+  const long long r = gridDim.x - 1 - blockIdx.x;
   const Row<T, VEC> row(logits + r * row_stride, classes);
   const float c = inv_t * kLog2e;
   T* out = grad + r * classes;
@@ -515,18 +657,25 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
     for (int e = tid; e < row.edges(); e += THREADS) out[row.edge(e)] = fill;
     return;
   }
-  const float coef = s.coef * g;
-  for (int v = tid; v < row.body; v += THREADS) {
-    const DfdVec<T, VEC> x = row.load(v);
-    DfdVec<T, VEC> o;
+  if (s.m_rest > kDeep) {
+    const float mc = s.m_rest * c;
+    const float coef = s.coef * g * exp2_fast(-__builtin_fmaf(s.m_rest, c, -mc));
+    stream<THREADS>(row, [&](const DfdVec<T, VEC>& x, int v) {
+      float z[VEC];
+      to_floats(x, z);
+      DfdVec<T, VEC> o;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
-      o.v[i] = DfdCvt<T>::from_f32(exp2_fast((DfdCvt<T>::to_f32(x.v[i]) - s.m_rest) * c) * coef);
-    dfd_vstore<T, VEC>(out + row.first(v), o);
-  }
-  for (int e = tid; e < row.edges(); e += THREADS) {
-    const int i = row.edge(e);
-    out[i] = DfdCvt<T>::from_f32(exp2_fast((row.at(i) - s.m_rest) * c) * coef);
+      for (int i = 0; i < VEC; ++i)
+        o.v[i] = DfdCvt<T>::from_f32(exp2_fast(__builtin_fmaf(z[i], c, -mc)) * coef);
+      store_once<T, VEC>(out + row.first(v), o);
+    });
+    for (int e = tid; e < row.edges(); e += THREADS) {
+      const int i = row.edge(e);
+      out[i] = DfdCvt<T>::from_f32(exp2_fast(__builtin_fmaf(row.at(i), c, -mc)) * coef);
+    }
+  } else {  // m_rest * c may be beyond fp32
+    for (int i = tid; i < classes; i += THREADS)
+      out[i] = DfdCvt<T>::from_f32(exp2_fast((row.at(i) - s.m_rest) * c) * (s.coef * g));
   }
   // the named classes' gradients take the place of what was just written
   __syncthreads();
@@ -553,19 +702,23 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
     case LogitType::kBf16: { using T = __hip_bfloat16; __VA_ARGS__; break; } \
     case LogitType::kF16: { using T = __half; __VA_ARGS__; break; }          \
   }
-#define ROW_THREADS(VAL, ...)                                    \
-  switch (VAL) {                                                 \
-    case 64: { constexpr int N = 64; __VA_ARGS__; break; }       \
-    case 256: { constexpr int N = 256; __VA_ARGS__; break; }     \
-    default: { constexpr int N = 1024; __VA_ARGS__; break; }     \
+#define ROW_THREADS(VAL, LARGEST, ...)                                  \
+  switch (VAL) {                                                        \
+    case 64: { constexpr int N = 64; __VA_ARGS__; break; }              \
+    case 256: { constexpr int N = 256; __VA_ARGS__; break; }            \
+    default: { constexpr int N = LARGEST; __VA_ARGS__; break; }         \
   }
 
 }  // namespace
 
 hipError_t topk_logits_launch(const TopkArgs& a, hipStream_t stream) {
-  const int threads = a.classes <= 4096 && a.k <= 32 ? 64 : a.classes <= 16384 && a.k <= 128 ? 256 : 1024;
+  // A wave alone has no barriers to wait at, more threads shorten a row's own
+  // time. bf16, k = 30, 1536 x 4096: 15 us by 64 threads, 21 by 256, 34 by 512;
+  // k = 64, 4096 x 65536: 140 us by 256, 163 by 512; 200 x 65536: 26 us by 256,
+  // 22 by 512. With k near the number of threads their bound is loose.
+  const int threads = a.classes <= 4096 && a.k <= 32 ? 64 : a.rows <= 256 || a.k > 160 ? 512 : 256;
   const float inv_t = 1.f / a.temperature;
-  LOGIT_TYPE(a.type, ROW_THREADS(threads, {
+  LOGIT_TYPE(a.type, ROW_THREADS(threads, 512, {
                constexpr int V = 16 / sizeof(T);
                topk_kernel<T, V, N><<<dim3((unsigned)a.rows), N, 0, stream>>>(
                    static_cast<const T*>(a.logits), a.row_stride, a.classes, a.k, inv_t,
@@ -575,10 +728,12 @@ hipError_t topk_logits_launch(const TopkArgs& a, hipStream_t stream) {
 }
 
 hipError_t distill_fwd(const DistillArgs& a, hipStream_t stream) {
-  const int threads = a.classes <= 2048 ? 64 : a.classes <= 16384 ? 256 : 1024;
+  // bf16: 1536 x 2048: 10.5 us by 64 threads, 11.4 by 256; 8192 x 32000: 147 us
+  // by 256, 170 by 64; 32 x 131072: 24 us by 256, 18 by 512, 17 by 1024.
+  const int threads = a.classes <= 4096 ? 64 : a.rows <= 512 ? 512 : 256;
   const float inv_t = 1.f / a.temperature;
   const int bytes = (a.classes + 16 + 31) / 32 * 4;
-  LOGIT_TYPE(a.type, ROW_THREADS(threads, {
+  LOGIT_TYPE(a.type, ROW_THREADS(threads, 512, {
                constexpr int V = 16 / sizeof(T);
                distill_fwd_kernel<T, V, N><<<dim3((unsigned)a.rows), N, bytes, stream>>>(
                    static_cast<const T*>(a.logits), a.row_stride, a.classes, a.k, inv_t,
@@ -589,9 +744,11 @@ hipError_t distill_fwd(const DistillArgs& a, hipStream_t stream) {
 }
 
 hipError_t distill_bwd(const DistillArgs& a, hipStream_t stream) {
-  const int threads = a.classes <= 2048 ? 64 : a.classes <= 16384 ? 256 : 1024;
+  // bf16: 1536 x 1000: 4.6 us by 64 threads, 4.5 by 256, 7.4 by 1024; 1024 x
+  // 16384: 13 us by 256, 15 by 64; 8192 x 32000: 212 us by 256, 178 by 1024.
+  const int threads = a.classes <= 1024 ? 64 : a.classes <= 16384 ? 256 : 1024;
   const float inv_t = 1.f / a.temperature;
-  LOGIT_TYPE(a.type, ROW_THREADS(threads, {
+  LOGIT_TYPE(a.type, ROW_THREADS(threads, 1024, {
                constexpr int V = 16 / sizeof(T);
                const T* z = static_cast<const T*>(a.logits);
                T* grad = static_cast<T*>(a.grad);

@@ -309,6 +309,10 @@ def special_answers(device, dtype, classes=1203, k=6):
     indices[11, 4] = indices[11, 1]      # a class that is named twice
     indices[12, :] = indices[12, 0]      # and one that is named by all
     z[13, 5] = 80.0                      # nearly certain
+    low_row = torch.full_like(z[:1], low)  # all others at the type's lowest value
+    low_row[0, indices[3, 0]] = 1.0
+    z = torch.cat([z, low_row])
+    values, indices, rest = (torch.cat([t, t[3:4]]) for t in (values, indices, rest))
     return z, values, indices, rest
 
 
