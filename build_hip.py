@@ -19,7 +19,7 @@ OUT_SO = os.path.join(REPO, "deepfake_detection_amd", "_hip_ops.so")
 BUILD_DIR = os.path.join(REPO, "build", "hip")
 
 SOURCES = ["bn_act.hip", "normalize.hip", "pool.hip", "se.hip", "optim.hip", "dwconv.hip", "pwconv.hip", "stemconv.hip", "head.hip",
-           "group_norm.hip", "distill.hip", "small_batch.hip", "ext.hip"]
+           "group_norm.hip", "group_norm_slab.hip", "distill.hip", "small_batch.hip", "ext.hip"]
 
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 

@@ -35,5 +35,12 @@ struct GnArgs {
 
 long long gn_fwd_ws(const GnArgs& a);
 long long gn_bwd_ws(const GnArgs& a);
+// Launches the pass that suits the shape: see group_norm.hip.
 hipError_t gn_fwd(const GnArgs& a, hipStream_t stream);
 hipError_t gn_bwd(const GnArgs& a, hipStream_t stream);
+
+// Slabs in registers (group_norm_slab.hip). sums: [n, 2, c] floats, the images'
+// parts of dbias and dweight, or null.
+bool gn_slab_fits(const GnArgs& a, bool backward);
+hipError_t gn_slab_fwd(const GnArgs& a, hipStream_t stream);
+hipError_t gn_slab_bwd(const GnArgs& a, float* sums, hipStream_t stream);

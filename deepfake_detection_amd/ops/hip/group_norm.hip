@@ -9,6 +9,10 @@
 //
 //   dbias = sum g;  dweight = sum g h;  dx = rstd (weight g - (A + h B) / m)
 //
+// What a block can hold of an image is normed by one block in one launch
+// (group_norm_slab.hip); this file streams the rest: statistics, then their
+// use.
+//
 // An image is a row-major [hw, c] matrix. A thread owns VEC neighbouring
 // channels, keeps their coefficients in registers and streams rows; a block
 // takes cpb such channel slots times 256 / cpb rows at a time (DfdPlan). All
@@ -16,66 +20,33 @@
 // block and chunk, joined in a fixed order, without atomics, so a result is
 // the same every time.
 
-#include "common.h"
-#include "group_norm.h"
+#include "group_norm_device.h"
 
 namespace {
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 256, kGroupBlock = 512;
 
 struct GnPlan {
   int vec, cpb, ctiles, chunks, rows_per_chunk;
+  int span;  // groups that a tile of channels can reach into
 };
-
-bool gn_aligned(const void* p, int bytes) {
-  return (reinterpret_cast<unsigned long long>(p) % bytes) == 0;
-}
-
-int gn_elem(GnType t) { return t == GnType::kF32 ? 4 : 2; }
 
 GnPlan gn_plan(const GnArgs& a) {
-  const int es = gn_elem(a.type);
-  int vec = dfd_pick_vec(a.c, es);
-  const void* ptrs[] = {a.x, a.y, a.residual, a.dy, a.dx};
-  for (const void* p : ptrs)
-    while (vec > 1 && !gn_aligned(p, vec * es)) vec >>= 1;
-  const DfdPlan p = dfd_plan(a.c / vec, a.hw, a.n);
+  const int vec = gn_vec(a);
+  // A thread takes 16 rows at least, for a block's sums have a price: 32x336
+  // x38x38 bf16 takes 36 us forward with 16, 48 with 4. Where that leaves CUs
+  // without work it takes fewer: 1x480x75x75 fp16 23 us with 4, 26 with 16.
+  DfdPlan p = {};
+  for (int rows = 16; rows >= 4; rows /= 2) {
+    p = dfd_plan(a.c / vec, a.hw, a.n, rows);
+    if (a.n * p.chunks * p.ctiles >= 256) break;
+  }
+  if (p.rows_per_chunk > 1 << 20) p.rows_per_chunk = 1 << 20;  // div_small's range
   // rounding up the rows of a chunk can leave the last chunks without any
   const int chunks = (int)((a.hw + p.rows_per_chunk - 1) / p.rows_per_chunk);
-  return {vec, p.cpb, p.ctiles, chunks, p.rows_per_chunk};
+  const int cpg = a.c / a.groups;
+  return {vec, p.cpb, p.ctiles, chunks, p.rows_per_chunk, (p.cpb * vec + cpg - 2) / cpg + 1};
 }
-
-// (count, mean, sum of squares about the mean) of a set of values; joining
-// two such sets loses nothing to a large common offset, which a plain sum of
-// squares would.
-struct Moments {
-  float n, mean, m2;
-};
-
-DFD_DEV Moments join(const Moments& a, const Moments& b) {
-  const float n = a.n + b.n;
-  if (n == 0.f) return a;
-  const float d = b.mean - a.mean;
-  const float w = b.n / n;
-  return {n, a.mean + d * w, a.m2 + b.m2 + d * d * a.n * w};
-}
-
-// The norm's weight or bias, in fp32 or in a halved model's own type.
-struct Params {
-  const void* p;
-  GnType type;
-  DFD_DEV float at(int i, float otherwise) const {
-    if (p == nullptr) return otherwise;
-    switch (type) {
-      case GnType::kBf16:
-        return DfdCvt<__hip_bfloat16>::to_f32(static_cast<const __hip_bfloat16*>(p)[i]);
-      case GnType::kF16:
-        return DfdCvt<__half>::to_f32(static_cast<const __half*>(p)[i]);
-      default:
-        return static_cast<const float*>(p)[i];
-    }
-  }
-};
 
 struct Place {
   long long image;
@@ -85,11 +56,12 @@ struct Place {
 };
 
 // Which rows and channels a thread of the streaming kernels takes. Blocks run
-// over channel tiles first, then chunks of rows, then images.
+// over channel tiles first, then chunks of rows, then images; the kernels that
+// use the statistics run from the last to the first, for what was read last
+// for them may still be cached.
 template <int VEC>
-DFD_DEV Place gn_place(long long hw, int c, int cpb, int ctiles, int chunks, int rows) {
+DFD_DEV Place gn_place(int b, long long hw, int c, int cpb, int ctiles, int chunks, int rows) {
   Place p;
-  const int b = blockIdx.x;
   const int ct = b % ctiles;
   const int ch = (b / ctiles) % chunks;
   p.image = b / (ctiles * chunks);
@@ -104,93 +76,100 @@ DFD_DEV Place gn_place(long long hw, int c, int cpb, int ctiles, int chunks, int
   return p;
 }
 
-// part[image][chunk][c] = (mean, m2) of the chunk's rows.
-template <typename T, int VEC>
-__global__ __launch_bounds__(kBlock) void gn_stats_kernel(
-    const T* __restrict__ x, float2* __restrict__ part, long long hw, int c, int cpb,
-    int ctiles, int chunks, int rows) {
-  __shared__ float lm[kBlock * VEC], lv[kBlock * VEC], ln[kBlock];
-  const Place p = gn_place<VEC>(hw, c, cpb, ctiles, chunks, rows);
-  float s1[VEC] = {}, s2[VEC] = {}, pivot[VEC] = {};
-  float cnt = 0.f;
-  if (p.in && p.r0 + p.rg < p.r1) {
-    const T* base = x + p.image * hw * c + p.c0;
-    // about the thread's own first row: its values are of the set's own size
-    DfdVec<T, VEC> first = dfd_vload<T, VEC>(base + (p.r0 + p.rg) * c);
+// f(row, vectors..) for the thread's rows from r on, U at a time; rows beyond
+// the last load that one again and are dropped, so that the loads of a turn
+// are all in flight together.
+template <int U, typename T, int VEC, typename F>
+DFD_DEV void gn_rows(const T* __restrict__ p, const T* __restrict__ q, long long r,
+                     long long r1, int nrg, int c, F f) {
+  for (; r < r1; r += U * nrg) {
+    DfdVec<T, VEC> v[U], w[U];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) pivot[i] = DfdCvt<T>::to_f32(first.v[i]);
-    cnt = 1.f;
-    for (long long r = p.r0 + p.rg + p.nrg; r < p.r1; r += p.nrg) {
-      const DfdVec<T, VEC> v = dfd_vload<T, VEC>(base + r * c);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = DfdCvt<T>::to_f32(v.v[i]) - pivot[i];
-        s1[i] += d;
-        s2[i] += d * d;
-      }
-      cnt += 1.f;
+    for (int u = 0; u < U; ++u) {
+      const long long row = r + u * nrg < r1 ? r + u * nrg : r1 - 1;
+      v[u] = dfd_vload<T, VEC>(p + row * c);
+      if (q) w[u] = dfd_vload<T, VEC>(q + row * c);
     }
-  }
-  const int t = threadIdx.x;
-  const float inv = cnt > 0.f ? 1.f / cnt : 0.f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    lm[t * VEC + i] = pivot[i] + s1[i] * inv;
-    const float m2 = s2[i] - s1[i] * s1[i] * inv;
-    lv[t * VEC + i] = m2 < 0.f ? 0.f : m2;  // a NaN stays one
-  }
-  ln[t] = cnt;
-  __syncthreads();
-  for (int s = p.nrg; s > 1;) {
-    const int h = (s + 1) / 2;
-    if (p.rg + h < s) {
-      const int o = t + h * cpb;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const Moments m = join({ln[t], lm[t * VEC + i], lv[t * VEC + i]},
-                               {ln[o], lm[o * VEC + i], lv[o * VEC + i]});
-        lm[t * VEC + i] = m.mean;
-        lv[t * VEC + i] = m.m2;
-      }
-      ln[t] += ln[o];
-    }
-    __syncthreads();
-    s = h;
-  }
-  if (p.in && p.rg == 0) {
-    const long long chunk = blockIdx.x / ctiles;  // image * chunks + chunk
-    float2* out = part + chunk * c + p.c0;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = make_float2(lm[t * VEC + i], lv[t * VEC + i]);
+    for (int u = 0; u < U; ++u)
+      if (r + u * nrg < r1) f(r + u * nrg, v[u], w[u]);
   }
 }
 
-// One wave a group: joins the chunks' and channels' moments.
+template <int L>
+DFD_DEV void gn_store_groups(const Columns& sum, Moments* part, int g0, int g1, int cpg,
+                             int first, int width, int each) {
+  for (int g = g0 + threadIdx.x / L; g <= g1; g += kBlock / L) {
+    const int from = g * cpg > first ? (g * cpg - first) / each : 0;
+    const int to = (g + 1) * cpg < first + width ? ((g + 1) * cpg - first) / each : sum.cols;
+    const Moments m = sum.join_columns<L>(from, to - from);
+    if (threadIdx.x % L == 0) part[g - g0] = m;
+  }
+}
+
+// part[image][chunk][tile][span] = the moments that the chunk's rows and the
+// tile's channels have of each group the tile reaches into (at most span).
+template <typename T, int VEC>
+__global__ __launch_bounds__(kBlock) void gn_stats_kernel(
+    const T* __restrict__ x, Moments* __restrict__ part, long long hw, int c, int cpg, int cpb,
+    int ctiles, int chunks, int rows, int span) {
+  extern __shared__ float lds[];
+  const Place p = gn_place<VEC>(blockIdx.x, hw, c, cpb, ctiles, chunks, rows);
+  const int first = blockIdx.x % ctiles * cpb * VEC;  // the tile's channels
+  const int width = c - first < cpb * VEC ? c - first : cpb * VEC;
+  // a vector within one group is one column
+  const bool whole = cpg % VEC == 0;
+  const int each = whole ? VEC : 1;
+  Columns sum(lds, width / each, p.nrg, whole ? cpg / VEC : cpg);
+  const int here = (int)(p.r1 - p.r0);
+  if (p.in) {
+    float s1[VEC] = {}, s2[VEC] = {}, pivot[VEC] = {};
+    if (p.rg < here) {
+      const T* base = x + p.image * hw * c + p.c0;
+      // about the thread's own first row: its values are of the set's own size
+      const DfdVec<T, VEC> one = dfd_vload<T, VEC>(base + (p.r0 + p.rg) * c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) pivot[i] = DfdCvt<T>::to_f32(one.v[i]);
+      gn_rows<4, T, VEC>(base, nullptr, p.r0 + p.rg + p.nrg, p.r1, p.nrg, c,
+                         [&](long long, const DfdVec<T, VEC>& v, const DfdVec<T, VEC>&) {
+#pragma unroll
+                           for (int i = 0; i < VEC; ++i) {
+                             const float d = DfdCvt<T>::to_f32(v.v[i]) - pivot[i];
+                             s1[i] += d;
+                             s2[i] += d * d;
+                           }
+                         });
+    }
+    sum.put<VEC>(p.rg, threadIdx.x % cpb, whole, sum.row_count(p.rg, here, 1), pivot, s1, s2);
+  }
+  sum.join_rows(here, each);
+  const int g0 = first / cpg, g1 = (first + width - 1) / cpg;
+  if (sum.small_groups(g1 - g0 + 1))
+    gn_store_groups<16>(sum, part + (long long)blockIdx.x * span, g0, g1, cpg, first, width, each);
+  else
+    gn_store_groups<kWave>(sum, part + (long long)blockIdx.x * span, g0, g1, cpg, first, width, each);
+}
+
+// One wave a group: joins the chunks' and tiles' moments.
 __global__ __launch_bounds__(kBlock) void gn_finalize_kernel(
-    const float2* __restrict__ part, float* __restrict__ mean, float* __restrict__ rstd,
-    long long total, long long hw, int c, int groups, int chunks, int rows, float eps) {
+    const Moments* __restrict__ part, float* __restrict__ mean, float* __restrict__ rstd,
+    long long total, int cpg, int groups, int tile, int ctiles, int chunks, int span,
+    float eps) {
   const long long id = (long long)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
   if (id >= total) return;
-  const int lane = threadIdx.x % kWave;
-  const int cpg = c / groups;
   const long long image = id / groups;
   const int g = (int)(id - image * groups);
-  const float2* src = part + image * chunks * c + (long long)g * cpg;
+  // the tiles that reach into the group
+  const int t0 = g * cpg / tile, tiles = (g * cpg + cpg - 1) / tile - t0 + 1;
   Moments m = {0.f, 0.f, 0.f};
-  for (int e = lane; e < chunks * cpg; e += kWave) {
-    const int ch = e / cpg;
-    const float2 v = src[(long long)ch * c + (e - ch * cpg)];
-    const long long left = hw - (long long)ch * rows;
-    m = join(m, {(float)(left < rows ? left : rows), v.x, v.y});
+  for (int e = threadIdx.x % kWave; e < chunks * tiles; e += kWave) {
+    const int ch = e / tiles, t = t0 + (e - ch * tiles);
+    m = join(m, part[((image * chunks + ch) * ctiles + t) * span + (g - t * tile / cpg)]);
   }
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) {
-    const Moments o = {__shfl_xor(m.n, off), __shfl_xor(m.mean, off), __shfl_xor(m.m2, off)};
-    m = lane & off ? join(o, m) : join(m, o);
-  }
-  if (lane == 0) {
+  m = lanes_join<kWave>(m);
+  if (threadIdx.x % kWave == 0) {
     mean[id] = m.mean;
-    rstd[id] = 1.f / sqrtf(m.m2 / m.n + eps);
+    rstd[id] = rsqrtf(m.m2 / m.n + eps);
   }
 }
 
@@ -200,7 +179,7 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(
     const T* __restrict__ residual, const float* __restrict__ drop, T* __restrict__ y,
     const float* __restrict__ mean, const float* __restrict__ rstd, long long hw, int c,
     int groups, int cpb, int ctiles, int chunks, int rows) {
-  const Place p = gn_place<VEC>(hw, c, cpb, ctiles, chunks, rows);
+  const Place p = gn_place<VEC>(gridDim.x - 1 - blockIdx.x, hw, c, cpb, ctiles, chunks, rows);
   if (!p.in) return;
   float mu[VEC], a[VEC], b[VEC];
   const int cpg = c / groups;
@@ -213,18 +192,18 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(
   }
   const float keep = drop ? drop[p.image] : 1.f;
   const long long off = p.image * hw * c + p.c0;
-  for (long long r = p.r0 + p.rg; r < p.r1; r += p.nrg) {
-    const DfdVec<T, VEC> v = dfd_vload<T, VEC>(x + off + r * c);
-    DfdVec<T, VEC> res, o;
-    if (residual) res = dfd_vload<T, VEC>(residual + off + r * c);
+  gn_rows<2, T, VEC>(
+      x + off, residual ? residual + off : nullptr, p.r0 + p.rg, p.r1, p.nrg, c,
+      [&](long long r, const DfdVec<T, VEC>& v, const DfdVec<T, VEC>& res) {
+        DfdVec<T, VEC> o;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float z = act_fwd((DfdCvt<T>::to_f32(v.v[i]) - mu[i]) * a[i] + b[i], ACT) * keep;
-      if (residual) z += DfdCvt<T>::to_f32(res.v[i]);
-      o.v[i] = DfdCvt<T>::from_f32(z);
-    }
-    dfd_vstore<T, VEC>(y + off + r * c, o);
-  }
+        for (int i = 0; i < VEC; ++i) {
+          float z = gn_act((DfdCvt<T>::to_f32(v.v[i]) - mu[i]) * a[i] + b[i], ACT) * keep;
+          if (residual) z += DfdCvt<T>::to_f32(res.v[i]);
+          o.v[i] = DfdCvt<T>::from_f32(z);
+        }
+        gn_store_once<T, VEC>(y + off + r * c, o);
+      });
 }
 
 // part[image][chunk][2][c] = sum g, sum g (x - mean) over the chunk's rows.
@@ -235,7 +214,7 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(
     const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part,
     long long hw, int c, int groups, int cpb, int ctiles, int chunks, int rows) {
   __shared__ float l1[kBlock * VEC], l2[kBlock * VEC];
-  const Place p = gn_place<VEC>(hw, c, cpb, ctiles, chunks, rows);
+  const Place p = gn_place<VEC>(blockIdx.x, hw, c, cpb, ctiles, chunks, rows);
   float s1[VEC] = {}, s2[VEC] = {};
   if (p.in) {
     float mu[VEC], a[VEC], b[VEC];
@@ -249,17 +228,17 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(
     }
     const float keep = drop ? drop[p.image] : 1.f;
     const long long off = p.image * hw * c + p.c0;
-    for (long long r = p.r0 + p.rg; r < p.r1; r += p.nrg) {
-      const DfdVec<T, VEC> v = dfd_vload<T, VEC>(x + off + r * c);
-      const DfdVec<T, VEC> u = dfd_vload<T, VEC>(dy + off + r * c);
+    gn_rows<2, T, VEC>(x + off, dy + off, p.r0 + p.rg, p.r1, p.nrg, c,
+                    [&](long long, const DfdVec<T, VEC>& v, const DfdVec<T, VEC>& u) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = DfdCvt<T>::to_f32(v.v[i]) - mu[i];
-        const float g = DfdCvt<T>::to_f32(u.v[i]) * keep * act_bwd(d * a[i] + b[i], ACT);
-        s1[i] += g;
-        s2[i] += g * d;
-      }
-    }
+                      for (int i = 0; i < VEC; ++i) {
+                        const float d = DfdCvt<T>::to_f32(v.v[i]) - mu[i];
+                        const float g = DfdCvt<T>::to_f32(u.v[i]) * keep *
+                                        gn_act_slope(d * a[i] + b[i], ACT);
+                        s1[i] += g;
+                        s2[i] += g * d;
+                      }
+                    });
   }
   const int t = threadIdx.x;
 #pragma unroll
@@ -292,65 +271,93 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(
   }
 }
 
-// One wave a group: k[image][group] = (A / m, B rstd / m), so that
-// dx = rstd (weight g - k.x - (x - mean) k.y).
-__global__ __launch_bounds__(kBlock) void gn_bwd_group_kernel(
-    const float* __restrict__ part, Params weight,
-    const float* __restrict__ rstd, float2* __restrict__ k, long long total, long long hw,
-    int c, int groups, int chunks) {
-  const long long id = (long long)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
-  if (id >= total) return;
-  const int lane = threadIdx.x % kWave;
+// A block takes some whole groups of an image, `width` channels: their sums
+// over the chunks,
+//   k[image][group] = (A / m, B rstd / m), so that
+//     dx = rstd (weight g - k.x - (x - mean) k.y)
+//   sums[image][2][c] = sum g, sum g h, if the parameters want them
+__global__ __launch_bounds__(kGroupBlock) void gn_bwd_group_kernel(
+    const float* __restrict__ part, Params weight, const float* __restrict__ rstd,
+    float2* __restrict__ k, float* __restrict__ sums, long long hw, int c, int groups,
+    int chunks, int width, int tiles) {
+  extern __shared__ float lds[];  // [2][parts * cols]
+  const long long image = blockIdx.x / tiles;
+  const int c0 = (int)(blockIdx.x % tiles) * width;
+  const int cols = c - c0 < width ? c - c0 : width;
   const int cpg = c / groups;
-  const long long image = id / groups;
-  const int g = (int)(id - image * groups);
-  const float* src = part + image * chunks * 2 * c + (long long)g * cpg;
-  float a = 0.f, b = 0.f;
-  for (int e = lane; e < chunks * cpg; e += kWave) {
-    const int ch = e / cpg, j = e - ch * cpg;
-    const float w = weight.at(g * cpg + j, 1.f);
-    a += w * src[(long long)ch * 2 * c + j];
-    b += w * src[(long long)ch * 2 * c + c + j];
+  const int parts = cols < kGroupBlock ? kGroupBlock / cols : 1;
+  const float* src = part + image * chunks * 2 * c + c0;
+  for (int i = threadIdx.x; i < parts * cols; i += kGroupBlock) {
+    const int p = i / cols, col = i - p * cols;
+    float a = 0.f, b = 0.f;
+#pragma unroll 4
+    for (int ch = p; ch < chunks; ch += parts) {
+      a += src[(long long)ch * 2 * c + col];
+      b += src[(long long)ch * 2 * c + c + col];
+    }
+    lds[i] = a;
+    lds[parts * cols + i] = b;
   }
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) {
-    a += __shfl_xor(a, off);
-    b += __shfl_xor(b, off);
-  }
-  if (lane == 0) {
-    const float m = (float)hw * (float)cpg;
-    const float r = rstd[id];
-    k[id] = make_float2(a / m, b * r * r / m);
+  __syncthreads();
+  if (sums)
+    for (int col = threadIdx.x; col < cols; col += kGroupBlock) {
+      float a = 0.f, b = 0.f;
+      for (int p = 0; p < parts; ++p) {
+        a += lds[p * cols + col];
+        b += lds[(parts + p) * cols + col];
+      }
+      float* out = sums + image * 2 * c + c0 + col;
+      out[0] = a;
+      out[c] = b * rstd[image * groups + (c0 + col) / cpg];
+    }
+  const int lane = threadIdx.x % kWave;
+  for (int g = threadIdx.x / kWave; g < cols / cpg; g += kGroupBlock / kWave) {
+    float a = 0.f, b = 0.f;
+    for (int e = lane; e < parts * cpg; e += kWave) {
+      const int p = e / cpg, col = g * cpg + (e - p * cpg);
+      const float w = weight.at(c0 + col, 1.f);
+      a += w * lds[p * cols + col];
+      b += w * lds[(parts + p) * cols + col];
+    }
+    a = lanes_sum<kWave>(a);
+    b = lanes_sum<kWave>(b);
+    if (lane == 0) {
+      const long long id = image * groups + c0 / cpg + g;
+      const float m = (float)hw * (float)cpg;
+      const float r = rstd[id];
+      k[id] = make_float2(a / m, b * r * r / m);
+    }
   }
 }
 
-// dweight[c], dbias[c]: 32 channels a block, 8 threads for each of them.
-__global__ __launch_bounds__(kBlock) void gn_bwd_params_kernel(
-    const float* __restrict__ part, const float* __restrict__ rstd,
-    float* __restrict__ dweight, float* __restrict__ dbias, long long n, int c, int groups,
-    int chunks) {
-  __shared__ float l1[kBlock], l2[kBlock];
+// dbias[c], dweight[c] from the images' sums: 32 channels a block, 32 threads
+// for each of them.
+__global__ __launch_bounds__(1024) void gn_bwd_params_kernel(
+    const float* __restrict__ sums, float* __restrict__ dweight, float* __restrict__ dbias,
+    long long n, int c) {
+  __shared__ float l1[1024], l2[1024];
   const int t = threadIdx.x;
   const int ch = blockIdx.x * 32 + t % 32;
   float s1 = 0.f, s2 = 0.f;
   if (ch < c) {
-    const int g = ch / (c / groups);
-    for (long long e = t / 32; e < n * chunks; e += 8) {
-      const float* src = part + e * 2 * c + ch;
-      s1 += src[0];
-      s2 += src[c] * rstd[e / chunks * groups + g];
+#pragma unroll 4
+    for (long long i = t / 32; i < n; i += 32) {
+      s1 += sums[i * 2 * c + ch];
+      s2 += sums[i * 2 * c + c + ch];
     }
   }
   l1[t] = s1;
   l2[t] = s2;
-  __syncthreads();
-  if (t < 32 && ch < c) {
-    for (int i = 1; i < 8; ++i) {
-      s1 += l1[t + 32 * i];
-      s2 += l2[t + 32 * i];
+  for (int h = 512; h >= 32; h /= 2) {
+    __syncthreads();
+    if (t < h) {
+      l1[t] += l1[t + h];
+      l2[t] += l2[t + h];
     }
-    if (dbias) dbias[ch] = s1;
-    if (dweight) dweight[ch] = s2;
+  }
+  if (t < 32 && ch < c) {
+    if (dbias) dbias[ch] = l1[t];
+    if (dweight) dweight[ch] = l2[t];
   }
 }
 
@@ -361,7 +368,7 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_dx_kernel(
     const float* __restrict__ mean, const float* __restrict__ rstd,
     const float2* __restrict__ k, T* __restrict__ dx, long long hw, int c, int groups,
     int cpb, int ctiles, int chunks, int rows) {
-  const Place p = gn_place<VEC>(hw, c, cpb, ctiles, chunks, rows);
+  const Place p = gn_place<VEC>(gridDim.x - 1 - blockIdx.x, hw, c, cpb, ctiles, chunks, rows);
   if (!p.in) return;
   float mu[VEC], a[VEC], b[VEC], k0[VEC], k1[VEC];
   const int cpg = c / groups;
@@ -378,62 +385,52 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_dx_kernel(
   }
   const float keep = drop ? drop[p.image] : 1.f;
   const long long off = p.image * hw * c + p.c0;
-  for (long long r = p.r0 + p.rg; r < p.r1; r += p.nrg) {
-    const DfdVec<T, VEC> v = dfd_vload<T, VEC>(x + off + r * c);
-    const DfdVec<T, VEC> u = dfd_vload<T, VEC>(dy + off + r * c);
-    DfdVec<T, VEC> o;
+  gn_rows<2, T, VEC>(x + off, dy + off, p.r0 + p.rg, p.r1, p.nrg, c,
+                  [&](long long r, const DfdVec<T, VEC>& v, const DfdVec<T, VEC>& u) {
+                    DfdVec<T, VEC> o;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float d = DfdCvt<T>::to_f32(v.v[i]) - mu[i];
-      const float g = DfdCvt<T>::to_f32(u.v[i]) * keep * act_bwd(d * a[i] + b[i], ACT);
-      o.v[i] = DfdCvt<T>::from_f32(g * a[i] - k0[i] - d * k1[i]);
-    }
-    dfd_vstore<T, VEC>(dx + off + r * c, o);
-  }
+                    for (int i = 0; i < VEC; ++i) {
+                      const float d = DfdCvt<T>::to_f32(v.v[i]) - mu[i];
+                      const float g = DfdCvt<T>::to_f32(u.v[i]) * keep *
+                                      gn_act_slope(d * a[i] + b[i], ACT);
+                      o.v[i] = DfdCvt<T>::from_f32(g * a[i] - k0[i] - d * k1[i]);
+                    }
+                    gn_store_once<T, VEC>(dx + off + r * c, o);
+                  });
 }
-
-#define GN_VEC(VAL, ...)                                    \
-  switch (VAL) {                                            \
-    case 8: { constexpr int V = 8; __VA_ARGS__; break; }    \
-    case 4: { constexpr int V = 4; __VA_ARGS__; break; }    \
-    case 2: { constexpr int V = 2; __VA_ARGS__; break; }    \
-    default: { constexpr int V = 1; __VA_ARGS__; break; }   \
-  }
-#define GN_TYPE(VAL, ...)                                            \
-  switch (VAL) {                                                     \
-    case GnType::kF32: { using T = float; __VA_ARGS__; break; }      \
-    case GnType::kBf16: { using T = __hip_bfloat16; __VA_ARGS__; break; } \
-    case GnType::kF16: { using T = __half; __VA_ARGS__; break; }     \
-  }
-#define GN_ACT(VAL, ...)                                                      \
-  switch (static_cast<Act>(VAL)) {                                            \
-    case Act::kRelu: { constexpr Act A = Act::kRelu; __VA_ARGS__; break; }    \
-    case Act::kSilu: { constexpr Act A = Act::kSilu; __VA_ARGS__; break; }    \
-    default: { constexpr Act A = Act::kNone; __VA_ARGS__; break; }            \
-  }
 
 }  // namespace
 
-long long gn_fwd_ws(const GnArgs& a) { return a.n * gn_plan(a).chunks * a.c * 2; }
+long long gn_fwd_ws(const GnArgs& a) {
+  if (gn_slab_fits(a, false)) return 0;
+  const GnPlan p = gn_plan(a);
+  return a.n * p.chunks * p.ctiles * p.span * (long long)(sizeof(Moments) / sizeof(float));
+}
 
+// The images' sums for the parameters; streaming, the chunks' and groups' too.
 long long gn_bwd_ws(const GnArgs& a) {
-  return a.n * gn_plan(a).chunks * a.c * 2 + a.n * a.groups * 2;
+  const long long sums = a.n * 2 * a.c;
+  return gn_slab_fits(a, true) ? sums : sums + a.n * gn_plan(a).chunks * a.c * 2 + a.n * a.groups * 2;
 }
 
 hipError_t gn_fwd(const GnArgs& a, hipStream_t stream) {
+  if (gn_slab_fits(a, false)) return gn_slab_fwd(a, stream);
   const GnPlan p = gn_plan(a);
   const Params weight = {a.weight, a.ptype}, bias = {a.bias, a.ptype};
   const dim3 grid((unsigned)(a.n * p.chunks * p.ctiles));
   const long long groups = a.n * a.groups;
   const dim3 waves((unsigned)((groups + 3) / 4));
+  const int cpg = a.c / a.groups;
+  const int cols = p.cpb * (cpg % p.vec == 0 ? 1 : p.vec);
+  const int lds = columns_lds(kBlock, kBlock / p.cpb, cols);
   GN_TYPE(a.type, GN_VEC(p.vec, {
             const T* x = static_cast<const T*>(a.x);
-            gn_stats_kernel<T, V><<<grid, kBlock, 0, stream>>>(
-                x, reinterpret_cast<float2*>(a.ws), a.hw, a.c, p.cpb, p.ctiles, p.chunks,
-                p.rows_per_chunk);
+            gn_stats_kernel<T, V><<<grid, kBlock, lds, stream>>>(
+                x, reinterpret_cast<Moments*>(a.ws), a.hw, a.c, cpg, p.cpb, p.ctiles,
+                p.chunks, p.rows_per_chunk, p.span);
             gn_finalize_kernel<<<waves, kBlock, 0, stream>>>(
-                reinterpret_cast<const float2*>(a.ws), a.mean, a.rstd, groups, a.hw, a.c,
-                a.groups, p.chunks, p.rows_per_chunk, a.eps);
+                reinterpret_cast<const Moments*>(a.ws), a.mean, a.rstd, groups, cpg, a.groups,
+                p.cpb * p.vec, p.ctiles, p.chunks, p.span, a.eps);
             GN_ACT(a.act, gn_apply_kernel<T, V, A><<<grid, kBlock, 0, stream>>>(
                               x, weight, bias, static_cast<const T*>(a.residual), a.drop,
                               static_cast<T*>(a.y), a.mean, a.rstd, a.hw, a.c, a.groups, p.cpb,
@@ -443,29 +440,38 @@ hipError_t gn_fwd(const GnArgs& a, hipStream_t stream) {
 }
 
 hipError_t gn_bwd(const GnArgs& a, hipStream_t stream) {
-  const GnPlan p = gn_plan(a);
-  const Params weight = {a.weight, a.ptype}, bias = {a.bias, a.ptype};
-  const dim3 grid((unsigned)(a.n * p.chunks * p.ctiles));
-  const long long groups = a.n * a.groups;
-  const dim3 waves((unsigned)((groups + 3) / 4));
-  float2* k = reinterpret_cast<float2*>(a.ws + a.n * p.chunks * a.c * 2);
-  GN_TYPE(a.type, GN_VEC(p.vec, GN_ACT(a.act, {
-            const T* x = static_cast<const T*>(a.x);
-            const T* dy = static_cast<const T*>(a.dy);
-            gn_bwd_sums_kernel<T, V, A><<<grid, kBlock, 0, stream>>>(
-                dy, x, weight, bias, a.drop, a.mean, a.rstd, a.ws, a.hw, a.c, a.groups,
-                p.cpb, p.ctiles, p.chunks, p.rows_per_chunk);
-            if (a.dweight || a.dbias)
-              gn_bwd_params_kernel<<<dim3((a.c + 31) / 32), kBlock, 0, stream>>>(
-                  a.ws, a.rstd, a.dweight, a.dbias, a.n, a.c, a.groups, p.chunks);
-            if (a.dx) {
-              gn_bwd_group_kernel<<<waves, kBlock, 0, stream>>>(
-                  a.ws, weight, a.rstd, k, groups, a.hw, a.c, a.groups, p.chunks);
-              gn_bwd_dx_kernel<T, V, A><<<grid, kBlock, 0, stream>>>(
-                  dy, x, weight, bias, a.drop, a.mean, a.rstd, k,
-                  static_cast<T*>(a.dx), a.hw, a.c, a.groups, p.cpb, p.ctiles, p.chunks,
-                  p.rows_per_chunk);
-            }
-          })));
+  float* sums = a.dweight || a.dbias ? a.ws : nullptr;
+  if (gn_slab_fits(a, true)) {
+    const hipError_t e = gn_slab_bwd(a, sums, stream);
+    if (e != hipSuccess) return e;
+  } else {
+    const GnPlan p = gn_plan(a);
+    const Params weight = {a.weight, a.ptype}, bias = {a.bias, a.ptype};
+    const dim3 grid((unsigned)(a.n * p.chunks * p.ctiles));
+    float2* k = reinterpret_cast<float2*>(a.ws + a.n * 2 * a.c);
+    float* part = a.ws + a.n * 2 * a.c + a.n * a.groups * 2;
+    // whole groups of about 32 channels: many blocks, and many threads a
+    // channel, since the chunks are read one after another
+    const int cpg = a.c / a.groups;
+    const int width = cpg >= 32 ? cpg : 32 / cpg * cpg;
+    const int tiles = (a.c + width - 1) / width;
+    const int lds = 2 * (int)sizeof(float) * (width > kGroupBlock ? width : kGroupBlock);
+    GN_TYPE(a.type, GN_VEC(p.vec, GN_ACT(a.act, {
+              const T* x = static_cast<const T*>(a.x);
+              const T* dy = static_cast<const T*>(a.dy);
+              gn_bwd_sums_kernel<T, V, A><<<grid, kBlock, 0, stream>>>(
+                  dy, x, weight, bias, a.drop, a.mean, a.rstd, part, a.hw, a.c, a.groups,
+                  p.cpb, p.ctiles, p.chunks, p.rows_per_chunk);
+              gn_bwd_group_kernel<<<dim3((unsigned)(a.n * tiles)), kGroupBlock, lds, stream>>>(
+                  part, weight, a.rstd, k, sums, a.hw, a.c, a.groups, p.chunks, width, tiles);
+              if (a.dx)
+                gn_bwd_dx_kernel<T, V, A><<<grid, kBlock, 0, stream>>>(
+                    dy, x, weight, bias, a.drop, a.mean, a.rstd, k, static_cast<T*>(a.dx),
+                    a.hw, a.c, a.groups, p.cpb, p.ctiles, p.chunks, p.rows_per_chunk);
+            })));
+  }
+  if (sums)
+    gn_bwd_params_kernel<<<dim3((a.c + 31) / 32), 1024, 0, stream>>>(sums, a.dweight, a.dbias,
+                                                                     a.n, a.c);
   return hipGetLastError();
 }

@@ -29,6 +29,13 @@ SHAPES = [
     (2, 1, 1, 8, 9),
     (7, 56, 8, 37, 41),
     (1, 256, 4, 90, 91),   # fp32: fewer chunks of rows than were asked for
+    (64, 160, 32, 19, 19),
+    (3, 448, 32, 10, 10),
+    (4, 336, 16, 38, 38),
+    (2, 1300, 1, 9, 11),   # groups wider than a block's channels
+    (1, 4096, 2, 23, 25),
+    (1, 16400, 16, 2, 3),
+    (1, 16, 4, 270, 260),  # more rows than a slab's indexes take
 ]
 
 
@@ -57,8 +64,12 @@ def oracle(x, groups, weight, bias, eps, act, residual, drop, dy):
     a, da = {"none": (z, torch.ones_like(z)), "relu": (z.clamp(min=0), (z > 0).double()),
              "silu": (z * sig, sig * (1 + z * (1 - sig)))}[act]
     y = a * keep + (0 if residual is None else residual)
+    # hat's own error does not shrink with it: the mean is a rounded sum of
+    # values about mu, whose mean size E|x - mu| r <= sqrt(E(x - mu)^2) r <= 1
+    # in hat's units, so hat is made of terms of 1 + |mu r| besides itself
+    hat_size = hat.abs() + mu.abs() * r + 1
     # z is hat * weight + bias in 32 bits and act' <= 1.1
-    y_size = (hat * per_c(weight)).abs() + per_c(bias).abs() + (mu * r * per_c(weight)).abs()
+    y_size = hat_size * per_c(weight).abs() + per_c(bias).abs()
     y_size = (1 + z.abs()) * (y_size * keep + (0 if residual is None else residual.abs()))
     g = dy * keep * da
     gw = g * per_c(weight)
@@ -69,11 +80,11 @@ def oracle(x, groups, weight, bias, eps, act, residual, drop, dy):
     if act == "relu":
         g_size = g.abs()
     dx_size = r * (g_size * per_c(weight).abs() + mean(g_size * per_c(weight).abs())
-                   + (hat.abs() + mu.abs() * r) * mean(g_size * per_c(weight).abs() * (hat.abs() + mu.abs() * r)))
+                   + hat_size * mean(g_size * per_c(weight).abs() * hat_size))
     return {
         "y": (y, y_size), "dx": (dx, dx_size),
         "dweight": ((g * hat).sum((0, 2, 3)),
-                    (g_size * (hat.abs() + mu.abs() * r)).sum((0, 2, 3))),
+                    (g_size * hat_size).sum((0, 2, 3))),
         "dbias": (g.sum((0, 2, 3)), g_size.sum((0, 2, 3))),
     }
 
