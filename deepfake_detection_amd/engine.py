@@ -86,7 +86,7 @@ def train_epoch(epoch, model, loader, optimizer, loss_fn, args, device,
         if use_cuda:
             input = input.contiguous(memory_format=torch.channels_last)
 
-        if _use_fused_head(model, loss_fn, target, use_cuda):
+        if teacher is None and _use_fused_head(model, loss_fn, target, use_cuda):
             # fused classifier GEMM + CE (ops/head.py): pooled features go
             # through one autograd op returning (loss, logits). Single-GPU
             # only — DDP must run module.forward for its reducer hooks.

@@ -161,12 +161,11 @@ __global__ __launch_bounds__(kBlock) void gn_finalize_kernel(
   const int g = (int)(id - image * groups);
   // the tiles that reach into the group
   const int t0 = g * cpg / tile, tiles = (g * cpg + cpg - 1) / tile - t0 + 1;
-  Moments m = {0.f, 0.f, 0.f};
-  for (int e = threadIdx.x % kWave; e < chunks * tiles; e += kWave) {
-    const int ch = e / tiles, t = t0 + (e - ch * tiles);
-    m = join(m, part[((image * chunks + ch) * ctiles + t) * span + (g - t * tile / cpg)]);
-  }
-  m = lanes_join<kWave>(m);
+  const float inv_tiles = 1.f / (float)tiles;
+  const Moments m = gather<kWave>(chunks * tiles, [&](int e) {
+    const int ch = div_small(e, inv_tiles), t = t0 + (e - ch * tiles);
+    return part[((image * chunks + ch) * ctiles + t) * span + (g - t * tile / cpg)];
+  });
   if (threadIdx.x % kWave == 0) {
     mean[id] = m.mean;
     rstd[id] = rsqrtf(m.m2 / m.n + eps);

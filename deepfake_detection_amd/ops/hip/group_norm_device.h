@@ -34,20 +34,12 @@ struct Params {
   }
 };
 
-// (count, mean, sum of squares about the mean) of a set of values; joining
-// two such sets loses nothing to a large common offset, which a plain sum of
-// squares would.
+// (count, mean, sum of squares about the mean) of a set of values: sets can be
+// put together without losing anything to a large common offset, as plain sums
+// of squares would.
 struct Moments {
   float n, mean, m2;
 };
-
-DFD_DEV Moments join(const Moments& a, const Moments& b) {
-  const float n = a.n + b.n;
-  if (n == 0.f) return a;
-  const float d = b.mean - a.mean;
-  const float w = b.n * __builtin_amdgcn_rcpf(n);
-  return {n, a.mean + d * w, a.m2 + b.m2 + d * d * a.n * w};
-}
 
 // Values from another lane of a row of 16, and from lane L to all.
 template <int CTRL>
@@ -61,38 +53,46 @@ DFD_DEV float lane_of(float v) {
 }
 constexpr int kQuadXor1 = 0xb1, kQuadXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
 
-// Sums and joins over L lanes, 16 or the whole wave, always in the same order:
-// right in the first lane of each L.
+// The sum over L lanes (1, 16 or the wave), the same bits in each of them.
 template <int L>
 DFD_DEV float lanes_sum(float v) {
-  v += lane_move<kQuadXor1>(v);
-  v += lane_move<kQuadXor2>(v);
-  v += lane_move<kHalfMirror>(v);
-  v += lane_move<kMirror>(v);
+  if constexpr (L > 1) {
+    v += lane_move<kQuadXor1>(v);
+    v += lane_move<kQuadXor2>(v);
+    v += lane_move<kHalfMirror>(v);
+    v += lane_move<kMirror>(v);
+  }
   if constexpr (L == kWave)
     v = (lane_of<0>(v) + lane_of<16>(v)) + (lane_of<32>(v) + lane_of<48>(v));
   return v;
 }
 
-template <int CTRL>
-DFD_DEV Moments moved(const Moments& m) {
-  return {lane_move<CTRL>(m.n), lane_move<CTRL>(m.mean), lane_move<CTRL>(m.m2)};
-}
-template <int FROM>
-DFD_DEV Moments moments_of(const Moments& m) {
-  return {lane_of<FROM>(m.n), lane_of<FROM>(m.mean), lane_of<FROM>(m.m2)};
-}
-
-template <int L>
-DFD_DEV Moments lanes_join(Moments m) {
-  m = join(m, moved<kQuadXor1>(m));
-  m = join(m, moved<kQuadXor2>(m));
-  m = join(m, moved<kHalfMirror>(m));
-  m = join(m, moved<kMirror>(m));
-  if constexpr (L == kWave)
-    m = join(join(moments_of<0>(m), moments_of<16>(m)),
-             join(moments_of<32>(m), moments_of<48>(m)));
-  return m;
+// The moments of n sets together, get(0) .. get(n - 1), by L lanes: the mean
+// first and the squares about it after, where what rounding left the mean
+// beside the true one is seen and taken out. Two short loops of sums are
+// faster than one of joins, each of which waits for the one before.
+template <int L, typename F>
+DFD_DEV Moments gather(int n, F get) {
+  const int lane = L > 1 ? threadIdx.x % L : 0;
+  float cnt = 0.f, sum = 0.f;
+  for (int e = lane; e < n; e += L) {
+    const Moments m = get(e);
+    cnt += m.n;
+    sum += m.n * m.mean;
+  }
+  cnt = lanes_sum<L>(cnt);
+  const float inv = cnt > 0.f ? __builtin_amdgcn_rcpf(cnt) : 0.f;
+  const float mean = lanes_sum<L>(sum) * inv;
+  float by = 0.f, m2 = 0.f;
+  for (int e = lane; e < n; e += L) {
+    const Moments m = get(e);
+    const float d = m.mean - mean;
+    by += m.n * d;
+    m2 += m.m2 + m.n * d * d;
+  }
+  by = lanes_sum<L>(by);
+  m2 = lanes_sum<L>(m2) - by * by * inv;
+  return {cnt, mean + by * inv, m2 < 0.f ? 0.f : m2};  // a NaN stays one
 }
 
 // n / d for 0 <= n < 2^21 by one product: the quotient's error, n / d * 2^-22
@@ -118,7 +118,7 @@ struct Columns {
     parts = div_small(blockDim.x, 1.f / (float)cols);
     if (parts > nrg) parts = nrg;
     if (parts < 1) parts = 1;
-    part = raw + NV * nrg * cols;
+    part = raw + NV * (nrg * cols > 32 ? nrg * cols : 32);
     sums = part + NV * parts * cols;
     counts = sums + NV * groups;
   }
@@ -181,13 +181,19 @@ struct Columns {
   }
 
   DFD_DEV void join_rows(int hw, int each) {
+    // the first `longer` of the threads' rows took `most` rows, the others one less
+    const int most = div_small(hw - 1 + nrg, 1.f / (float)nrg);
+    const int longer = hw - (most - 1) * nrg;
+    const float inv_parts = 1.f / (float)parts;
     __syncthreads();
     const int p0 = cols > (int)blockDim.x ? 0 : div_small(threadIdx.x, 1.f / (float)cols);
     if (p0 < parts)
       for (int col = threadIdx.x - p0 * cols; col < cols; col += blockDim.x) {
-        Moments m = {0.f, 0.f, 0.f};
-        for (int r = p0; r < nrg; r += parts)
-          m = join(m, {row_count(r, hw, each), raw[r * cols + col], raw[(nrg + r) * cols + col]});
+        const Moments m = gather<1>(div_small(nrg - 1 - p0 + parts, inv_parts), [&](int e) {
+          const int r = p0 + e * parts;
+          const float n = (float)((r < longer ? most : most - 1) * each);
+          return Moments{n, raw[r * cols + col], raw[(nrg + r) * cols + col]};
+        });
         part[p0 * cols + col] = m.mean;
         part[(parts + p0) * cols + col] = m.m2;
         if (col == 0) counts[p0] = m.n;
@@ -195,62 +201,121 @@ struct Columns {
     __syncthreads();
   }
 
-  // The moments of columns c0 .. c0 + n, by L lanes.
+  // The moments of columns c0 .. c0 + n, by L lanes; of `of` waves that share
+  // the work, the one numbered `wave`.
   template <int L>
-  DFD_DEV Moments join_columns(int c0, int n) const {
-    Moments m = {0.f, 0.f, 0.f};
+  DFD_DEV Moments join_columns(int c0, int n, int wave = 0, int of = 1) const {
     const float inv_n = 1.f / (float)n;
-    for (int e = threadIdx.x % L; e < parts * n; e += L) {
+    const int all = parts * n;
+    const int each = of == 1 ? all : (all + of - 1) / of;  // a wave's entries
+    const int from = wave * each;
+    const int count = all - from < each ? all - from : each;
+    return gather<L>(count, [&](int i) {
+      const int e = from + i;
       const int p = div_small(e, inv_n);
       const int col = c0 + (e - p * n);
-      m = join(m, {counts[p], part[p * cols + col], part[(parts + p) * cols + col]});
-    }
-    return lanes_join<L>(m);
+      return Moments{counts[p], part[p * cols + col], part[(parts + p) * cols + col]};
+    });
   }
 
-  // Many small groups are taken by 16 lanes each, a few large ones by a wave.
+  // Many small groups are taken by 16 lanes each, a few large ones by a wave
+  // each or by several.
   DFD_DEV bool small_groups(int count) const { return count * kWave > (int)blockDim.x; }
+  DFD_DEV int waves_a_group() const {
+    const int w = (int)(blockDim.x / kWave) / groups;
+    return w < 1 ? 1 : w;
+  }
 
   // sums[0][group] = mean, sums[1][group] = 1 / sqrt(variance + eps).
-  template <int L>
-  DFD_DEV void join_groups_by(float eps) {
-    for (int g = threadIdx.x / L; g < groups; g += blockDim.x / L) {
-      const Moments m = join_columns<L>(g * cpg, cpg);
-      if (threadIdx.x % L == 0) {
-        sums[g] = m.mean;
-        sums[groups + g] = rsqrtf(m.m2 / m.n + eps);
+  DFD_DEV void join_groups(float eps) {
+    auto store = [&](int g, const Moments& m) {
+      sums[g] = m.mean;
+      sums[groups + g] = rsqrtf(m.m2 * __builtin_amdgcn_rcpf(m.n) + eps);
+    };
+    if (small_groups(groups)) {
+      for (int g = threadIdx.x / 16; g < groups; g += blockDim.x / 16) {
+        const Moments m = join_columns<16>(g * cpg, cpg);
+        if (threadIdx.x % 16 == 0) store(g, m);
+      }
+    } else {
+      const int per = waves_a_group();
+      const int g = threadIdx.x / kWave / per, w = threadIdx.x / kWave - g * per;
+      if (g < groups) {
+        const Moments m = join_columns<kWave>(g * cpg, cpg, w, per);
+        if (threadIdx.x % kWave == 0) {
+          if (per == 1) {
+            store(g, m);
+          } else {
+            float* to = raw + 3 * (g * per + w);  // the rows' sums have been read
+            to[0] = m.n;
+            to[1] = m.mean;
+            to[2] = m.m2;
+          }
+        }
+      }
+      if (per > 1) {
+        __syncthreads();
+        const int h = threadIdx.x / 16;
+        if (h < groups) {
+          const Moments m = gather<16>(per, [&](int e) {
+            const float* from = raw + 3 * (h * per + e);
+            return Moments{from[0], from[1], from[2]};
+          });
+          if (threadIdx.x % 16 == 0) store(h, m);
+        }
       }
     }
-  }
-  DFD_DEV void join_groups(float eps) {
-    if (small_groups(groups)) join_groups_by<16>(eps);
-    else join_groups_by<kWave>(eps);
     __syncthreads();
   }
 
-  // Sums over the columns of a group: sums[v][group].
+  // Sums over the columns of a group, weighted: sums[v][group].
   template <int L, typename W>
-  DFD_DEV void over_groups_by(W weight) {
-    for (int g = threadIdx.x / L; g < groups; g += blockDim.x / L) {
-      float s[NV] = {};
-      for (int e = threadIdx.x % L; e < parts * cpg; e += L) {
-        const int p = div_small(e, inv_cpg);
-        const int col = g * cpg + (e - p * cpg);
-        const float w = weight(col);
+  DFD_DEV void group_sum(int g, int wave, int of, W weight, float (&s)[NV]) const {
+    const int all = parts * cpg;
+    const int each = of == 1 ? all : (all + of - 1) / of;
+    const int end = (wave + 1) * each < all ? (wave + 1) * each : all;
+    for (int e = wave * each + threadIdx.x % L; e < end; e += L) {
+      const int p = div_small(e, inv_cpg);
+      const int col = g * cpg + (e - p * cpg);
+      const float w = weight(col);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) s[v] += w * part[(v * parts + p) * cols + col];
-      }
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        s[v] = lanes_sum<L>(s[v]);
-        if (threadIdx.x % L == 0) sums[v * groups + g] = s[v];
-      }
+      for (int v = 0; v < NV; ++v) s[v] += w * part[(v * parts + p) * cols + col];
     }
+#pragma unroll
+    for (int v = 0; v < NV; ++v) s[v] = lanes_sum<L>(s[v]);
   }
+
   template <typename W>
   DFD_DEV void over_groups(W weight) {
-    if (small_groups(groups)) over_groups_by<16>(weight);
-    else over_groups_by<kWave>(weight);
+    if (small_groups(groups)) {
+      for (int g = threadIdx.x / 16; g < groups; g += blockDim.x / 16) {
+        float s[NV] = {};
+        group_sum<16>(g, 0, 1, weight, s);
+        if (threadIdx.x % 16 == 0)
+#pragma unroll
+          for (int v = 0; v < NV; ++v) sums[v * groups + g] = s[v];
+      }
+    } else {
+      const int per = waves_a_group();
+      const int g = threadIdx.x / kWave / per, w = threadIdx.x / kWave - g * per;
+      if (g < groups) {
+        float s[NV] = {};
+        group_sum<kWave>(g, w, per, weight, s);
+        if (threadIdx.x % kWave == 0)
+#pragma unroll
+          for (int v = 0; v < NV; ++v) (per == 1 ? sums[v * groups + g] : raw[NV * (g * per + w) + v]) = s[v];
+      }
+      if (per > 1) {
+        __syncthreads();  // raw: the rows' sums have been read
+        if ((int)threadIdx.x < groups)
+#pragma unroll
+          for (int v = 0; v < NV; ++v) {
+            float s = 0.f;
+            for (int e = 0; e < per; ++e) s += raw[NV * (threadIdx.x * per + e) + v];
+            sums[v * groups + threadIdx.x] = s;
+          }
+      }
+    }
     __syncthreads();
   }
 };
@@ -259,7 +324,8 @@ struct Columns {
 // more.
 static inline int columns_lds(int threads, int nrg, int cols) {
   const int part = threads > cols ? threads : cols;  // at least parts * cols
-  return 8 * (nrg * cols + part + cols) + 4 * threads;
+  const int raw = nrg * cols > 32 ? nrg * cols : 32;  // also what 16 waves share
+  return 8 * (raw + part + cols) + 4 * threads;
 }
 
 // The activation and its derivative at z. The sigmoid's reciprocal is one

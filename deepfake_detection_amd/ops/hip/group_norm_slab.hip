@@ -10,10 +10,11 @@
 //
 // These are small shapes, where a launch's fixed costs count: the loops stay
 // rolled, since code that runs once costs more to fetch than to run. Forward,
-// 64x160x19x19 bf16 takes 12.4 us (two passes over rows in registers, all
-// unrolled: 17.4; streaming: 38 in three launches), 32x256x19x19 fp16 8.8 (its
-// 12 MB at the rate of a large copy: 2.4), 1x1632x10x10 fp16 8.5; what is left
-// is the chain of a block's loads, four barriers and stores.
+// 64x160x19x19 bf16 takes 12.0 us (two passes over rows in registers, all
+// unrolled: 17.4; streaming: 38 in three launches), 32x256x19x19 fp16 9.0 (its
+// 12 MB at the rate of a large copy: 2.4), 1x1632x10x10 fp16 7.6. What is left
+// is a block's chain: by a clock in the kernel 2.3 to 3.7 us until the rows are
+// there, 2.3 for the sums, 1.0 to 2.6 for the activation and its stores.
 
 #include "group_norm_device.h"
 
@@ -132,21 +133,28 @@ __global__ __launch_bounds__(kMaxThreads) void gn_slab_fwd_kernel(
     weight.load<VEC>(s.c0 + s.slot * VEC, 1.f, ka);
     bias.load<VEC>(s.c0 + s.slot * VEC, 0.f, kb);
     float pivot[VEC] = {}, a[VEC] = {}, b[VEC] = {};
-    if (s.rg < hw) {
-      const DfdVec<T, VEC> v = dfd_vload<T, VEC>(x + base + (long long)s.rg * c);
-      data[s.rg * nslots + s.slot] = v;
+    constexpr int U = 4;  // loads in flight; those beyond the rows are dropped
+    for (int row = s.rg; row < hw; row += U * nrg) {
+      DfdVec<T, VEC> v[U];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) pivot[i] = DfdCvt<T>::to_f32(v.v[i]);
-    }
-#pragma unroll 4
-    for (int row = s.rg + nrg; row < hw; row += nrg) {
-      const DfdVec<T, VEC> v = dfd_vload<T, VEC>(x + base + (long long)row * c);
-      data[row * nslots + s.slot] = v;
+      for (int u = 0; u < U; ++u) {
+        const int r = row + u * nrg < hw ? row + u * nrg : row;
+        v[u] = dfd_vload<T, VEC>(x + base + (long long)r * c);
+      }
+      if (row == s.rg) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = DfdCvt<T>::to_f32(v.v[i]) - pivot[i];
-        a[i] += d;
-        b[i] += d * d;
+        for (int i = 0; i < VEC; ++i) pivot[i] = DfdCvt<T>::to_f32(v[0].v[i]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (row + u * nrg >= hw) continue;
+        data[(row + u * nrg) * nslots + s.slot] = v[u];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float d = DfdCvt<T>::to_f32(v[u].v[i]) - pivot[i];
+          a[i] += d;
+          b[i] += d * d;
+        }
       }
     }
     sum.put<VEC>(s.rg, s.slot, whole, sum.row_count(s.rg, hw, 1), pivot, a, b);

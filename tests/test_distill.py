@@ -546,6 +546,26 @@ def small_epoch(device):
     assert all(torch.equal(v, given[k]) for k, v in teacher.state_dict().items())
 
 
+def test_a_teacher_is_never_dropped():
+    """A loss that takes no teacher's output is refused, also where the step
+    would run through the fused head."""
+    from deepfake_detection_amd.engine import train_epoch
+
+    model = torch.nn.Sequential(torch.nn.Flatten(), torch.nn.Linear(12, 2))
+    args = types.SimpleNamespace(log_interval=1, recovery_interval=0, amp=False, prefetcher=True)
+    with pytest.raises(TypeError):
+        train_epoch(0, model, [(torch.randn(2, 3, 2, 2), torch.tensor([0, 1]))],
+                    torch.optim.SGD(model.parameters(), lr=0.1), torch.nn.CrossEntropyLoss(),
+                    args, torch.device("cpu"), teacher=model)
+
+
+def test_one_row_without_a_batch():
+    z = torch.randn(11).requires_grad_()
+    loss = O.distill_topk(z, *O.topk_logits(torch.randn(11), 3))
+    assert loss.shape == ()
+    assert torch.autograd.grad(loss, z)[0].shape == (11,)
+
+
 def test_training_epoch_cpu():
     small_epoch("cpu")
 

@@ -35,6 +35,8 @@ SHAPES = [
     (2, 1300, 1, 9, 11),   # groups wider than a block's channels
     (1, 4096, 2, 23, 25),
     (1, 16400, 16, 2, 3),
+    (66, 32, 4, 48, 48),   # bf16: a slab of nearly all of a block's LDS
+    (3, 4, 4, 1, 1),       # one value a group
     (1, 16, 4, 270, 260),  # more rows than a slab's indexes take
 ]
 
@@ -467,12 +469,13 @@ def test_offsets_beyond_32_bits():
 
 
 @pytest.mark.gpu
-def test_model_step_against_cpu():
+@pytest.mark.parametrize("name", ["efficientnet_b0", "resnet18"])
+def test_model_step_against_cpu(name):
     """A converted model's forward and gradients in fp32, GPU against CPU."""
     import deepfake_detection_amd as dfd
 
     torch.manual_seed(0)
-    model = convert_groupnorm_model(dfd.create_model("efficientnet_b0", num_classes=4))
+    model = convert_groupnorm_model(dfd.create_model(name, num_classes=4))
     model.eval()
     x = torch.randn(2, 3, 64, 64)
     want = model(x)
