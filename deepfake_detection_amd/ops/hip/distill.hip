@@ -180,12 +180,6 @@ template <> constexpr int key_bits<__half>() { return 19; }
 
 constexpr unsigned kOffKey = ~0xff800000u;  // the key of -inf
 
-template <int THREADS>
-DFD_DEV int block_count(bool yes) {
-  if (THREADS == kWave) return __popcll(__ballot(yes));
-  return __syncthreads_count(yes);
-}
-
 // The place of each thread that says yes among them, in thread order.
 template <int THREADS>
 DFD_DEV int block_rank(bool yes, int* lds, int& total) {
@@ -213,9 +207,9 @@ DFD_DEV int block_rank(bool yes, int* lds, int& total) {
 // ---------------------------------------------------------------------------
 //
 // One pass over the row: every thread takes its vectors in up to kParts parts
-// and keeps the largest value and the sum of each. The k-th largest of the
-// threads' largest is at most the row's k-th largest: what lies below that
-// bound is not taken. Only the parts whose largest reaches it (about k of
+// and keeps the largest value and the sum of each. A key that k of the threads'
+// largest reach is at most the row's k-th largest: what lies below that bound
+// is not taken. Only the parts whose largest reaches it (about k of
 // them) hold candidates; their elements are read again, from the cache, by all
 // threads together, and sorted into candidates and rest. A candidate's rank is
 // the number of greater ones. -inf is no candidate (nothing is said of a class
@@ -238,18 +232,30 @@ struct TopkLds {
   unsigned short hot[THREADS * kParts];  // part * THREADS + thread
   Sum sums[THREADS / kWave];
   int counts[THREADS / kWave];
+  unsigned bounds[THREADS / kWave];
   int n;
 };
 
-// The largest key that at least k of the threads' keys reach.
+// A key that at least k of the threads' keys reach, near to the largest such:
+// each wave finds its own (k / waves)-th largest by counting lanes, bit by bit,
+// and the least of these is taken. (The block's k-th largest itself takes a
+// barrier for each bit: by 256 threads 39 us for 2961 x 9591 fp16, k = 23, and
+// 31 so.)
 template <int THREADS, int BITS>
-DFD_DEV unsigned topk_bound(unsigned key, int k) {
+DFD_DEV unsigned topk_bound(unsigned key, int k, unsigned* lds) {
+  constexpr int kWaves = THREADS / kWave;
+  const int own = (k + kWaves - 1) / kWaves;
   unsigned bound = 0;
   for (int b = 31; b > 31 - BITS; --b) {
     const unsigned test = bound | (1u << b);
-    const int n = block_count<THREADS>(key >= test);
-    if (n >= k) bound = test;
-    if (n == k) break;
+    const int n = __popcll(__ballot(key >= test));
+    if (n >= own) bound = test;
+    if (n == own) break;
+  }
+  if (kWaves > 1) {
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = bound;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) bound = lds[w] < bound ? lds[w] : bound;
   }
   // the bits that a narrow type does not have are ones in a negative value's key
   return bound >> 31 ? bound : bound | (unsigned)((1ull << (32 - BITS)) - 1);
@@ -394,7 +400,7 @@ __global__ __launch_bounds__(THREADS) void topk_kernel(
     }
   }
   if (tid == 0) lds.n = 0;
-  const unsigned bound = topk_bound<THREADS, kBits>(key, k);
+  const unsigned bound = topk_bound<THREADS, kBits>(key, k, lds.bounds);
 
   // the hot parts' list, in a fixed order; the sum of the others
   Sum mine = {kLowest, 0.f};
@@ -711,19 +717,40 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
 
 }  // namespace
 
-hipError_t topk_logits_launch(const TopkArgs& a, hipStream_t stream) {
-  // A wave alone has no barriers to wait at, more threads shorten a row's own
-  // time. bf16, k = 30, 1536 x 4096: 15 us by 64 threads, 21 by 256, 34 by 512;
-  // k = 64, 4096 x 65536: 140 us by 256, 163 by 512; 200 x 65536: 26 us by 256,
-  // 22 by 512. With k near the number of threads their bound is loose.
-  const int threads = a.classes <= 4096 && a.k <= 32 ? 64 : a.rows <= 256 || a.k > 160 ? 512 : 256;
+template <typename T, int THREADS>
+static void topk_launch(const TopkArgs& a, hipStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const T* z = static_cast<const T*>(a.logits);
+  T* values = static_cast<T*>(a.values);
   const float inv_t = 1.f / a.temperature;
-  LOGIT_TYPE(a.type, ROW_THREADS(threads, 512, {
-               constexpr int V = 16 / sizeof(T);
-               topk_kernel<T, V, N><<<dim3((unsigned)a.rows), N, 0, stream>>>(
-                   static_cast<const T*>(a.logits), a.row_stride, a.classes, a.k, inv_t,
-                   static_cast<T*>(a.values), a.indices, a.rest);
-             }));
+  const dim3 grid((unsigned)a.rows);
+  // every thread has to have elements for the bound to be one
+  if (a.classes >= V * (THREADS + 1))
+    topk_kernel<T, V, THREADS><<<grid, THREADS, 0, stream>>>(
+        z, a.row_stride, a.classes, a.k, inv_t, values, a.indices, a.rest);
+  else
+    topk_kernel<T, 1, THREADS><<<grid, THREADS, 0, stream>>>(
+        z, a.row_stride, a.classes, a.k, inv_t, values, a.indices, a.rest);
+}
+
+hipError_t topk_logits_launch(const TopkArgs& a, hipStream_t stream) {
+  // A wave alone has no barriers to wait at, and many rows hide its own time;
+  // more threads shorten a row's. us by 64, 256 and 512 threads: bf16, k = 16,
+  // 4096 x 16000: 36, 44, 59; 4096 x 32000: 63, 65, 76; fp16, k = 12, 4929 x
+  // 3925: 20, 36, 60; k = 64, 4096 x 65536: -, 128, 138; fp32, k = 20, 100 x
+  // 10000: 15, 10, 10; bf16, 1 x 131072: -, 23, 19. A bound needs k / waves of a wave's
+  // 64 lanes, and fewer than half of them to be near: fp32, k = 250, 2000 x
+  // 10000: -, 638, 90.
+  const bool one_wave = a.k <= 32 && (a.classes <= 2048 || (a.rows >= 1024 && a.classes <= 32768));
+  const bool many = a.k > 160 || (a.rows <= 256 && a.classes > 16384);
+  const int threads = one_wave ? 64 : many ? 512 : 256;
+  LOGIT_TYPE(a.type, {
+    switch (threads) {
+      case 64: topk_launch<T, 64>(a, stream); break;
+      case 256: topk_launch<T, 256>(a, stream); break;
+      default: topk_launch<T, 512>(a, stream); break;
+    }
+  });
   return hipGetLastError();
 }
 
