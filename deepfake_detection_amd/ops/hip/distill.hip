@@ -91,6 +91,17 @@ struct Row {
     tail = n - head - body * VEC;
   }
   DFD_DEV DfdVec<T, VEC> load(int v) const { return dfd_vload<T, VEC>(p + head + (long long)v * VEC); }
+  DFD_DEV DfdVec<T, VEC> load_once(int v) const {
+    if constexpr (VEC * sizeof(T) == 16) {
+      typedef unsigned Words __attribute__((ext_vector_type(4)));
+      const Words w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(p + head + (long long)v * VEC));
+      DfdVec<T, VEC> x;
+      __builtin_memcpy(&x, &w, sizeof(x));
+      return x;
+    } else {
+      return load(v);
+    }
+  }
   DFD_DEV int first(int v) const { return head + v * VEC; }
   DFD_DEV int edges() const { return head + tail; }
   DFD_DEV int edge(int e) const { return e < head ? e : head + body * VEC + (e - head); }
@@ -99,8 +110,8 @@ struct Row {
 
 // f(vector, its number) for the thread's vectors of a row. Four loads are in
 // flight at a time; those beyond the row load its last vector again and are
-// dropped, which costs less than a branch around each.
-template <int THREADS, typename T, int VEC, typename F>
+// dropped, which costs less than a branch around each. ONCE: past the caches.
+template <int THREADS, bool ONCE, typename T, int VEC, typename F>
 DFD_DEV void stream(const Row<T, VEC>& row, F f) {
   constexpr int U = 4;
   for (int v = threadIdx.x; v < row.body; v += U * THREADS) {
@@ -108,7 +119,8 @@ DFD_DEV void stream(const Row<T, VEC>& row, F f) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int w = v + u * THREADS;
-      x[u] = row.load(w < row.body ? w : row.body - 1);
+      const int at = w < row.body ? w : row.body - 1;
+      x[u] = ONCE ? row.load_once(at) : row.load(at);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -503,7 +515,7 @@ static_assert(sizeof(RowStats) == kDistillStats * sizeof(float), "stats");
 
 constexpr float kTeaches = 0.f, kTwice = 1.f, kNothing = 2.f, kBadIndex = 3.f;
 
-template <typename T, int VEC, int THREADS>
+template <typename T, int VEC, int THREADS, bool ONCE>
 __global__ __launch_bounds__(THREADS) void distill_fwd_kernel(
     const T* __restrict__ logits, long long row_stride, int classes, int k, float inv_t,
     const void* __restrict__ values, LogitType vtype, const long long* __restrict__ indices,
@@ -553,7 +565,7 @@ __global__ __launch_bounds__(THREADS) void distill_fwd_kernel(
   };
   auto named_at = [&](int i) { return marks[(i + pad) / 8] >> ((i + pad) % 8) & 1; };
   FastSum fast(c);
-  stream<THREADS>(row, [&](const DfdVec<T, VEC>& x, int v) {
+  stream<THREADS, ONCE>(row, [&](const DfdVec<T, VEC>& x, int v) {
     if (marks_of(v)) return;
     float z[VEC];
     to_floats(x, z);
@@ -640,7 +652,7 @@ __global__ __launch_bounds__(THREADS) void distill_fwd_kernel(
   }
 }
 
-template <typename T, int VEC, int THREADS>
+template <typename T, int VEC, int THREADS, bool ONCE>
 __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
     const T* __restrict__ logits, long long row_stride, int classes, int k, float inv_t,
     const void* __restrict__ values, LogitType vtype, const long long* __restrict__ indices,
@@ -666,7 +678,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
   if (s.m_rest > kDeep) {
     const float mc = s.m_rest * c;
     const float coef = s.coef * g * exp2_fast(-__builtin_fmaf(s.m_rest, c, -mc));
-    stream<THREADS>(row, [&](const DfdVec<T, VEC>& x, int v) {
+    stream<THREADS, ONCE>(row, [&](const DfdVec<T, VEC>& x, int v) {
       float z[VEC];
       to_floats(x, z);
       DfdVec<T, VEC> o;
@@ -754,25 +766,40 @@ hipError_t topk_logits_launch(const TopkArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Logits that the 256 MB of cache hold are still there for the backward pass;
+// of larger ones the loads pass by it. Forward and backward us, so and
+// otherwise: 8192 x 32000 bf16 (524 MB) 92 + 180 and 123 + 176, 513 x 49999
+// fp32 (103 MB) 27 + 44 and 24 + 34.
+static bool past_caches(const DistillArgs& a) {
+  return a.rows * a.classes * (a.type == LogitType::kF32 ? 4 : 2) > 256ll << 20;
+}
+
 hipError_t distill_fwd(const DistillArgs& a, hipStream_t stream) {
-  // bf16: 1536 x 2048: 10.5 us by 64 threads, 11.4 by 256; 8192 x 32000: 147 us
-  // by 256, 170 by 64; 32 x 131072: 24 us by 256, 18 by 512, 17 by 1024.
+  // bf16: 1536 x 2048: 10.5 us by 64 threads, 11.4 by 256; 8192 x 32000 (all
+  // through the cache): 147 us by 256, 170 by 64; 32 x 131072: 24 us by 256, 18
+  // by 512, 17 by 1024.
   const int threads = a.classes <= 4096 ? 64 : a.rows <= 512 ? 512 : 256;
   const float inv_t = 1.f / a.temperature;
   const int bytes = (a.classes + 16 + 31) / 32 * 4;
+  const bool once = past_caches(a);
   LOGIT_TYPE(a.type, ROW_THREADS(threads, 512, {
                constexpr int V = 16 / sizeof(T);
-               distill_fwd_kernel<T, V, N><<<dim3((unsigned)a.rows), N, bytes, stream>>>(
-                   static_cast<const T*>(a.logits), a.row_stride, a.classes, a.k, inv_t,
-                   a.values, a.vtype, a.indices, a.rest, a.loss,
-                   reinterpret_cast<RowStats*>(a.stats));
+               auto launch = [&](auto kernel) {
+                 kernel<<<dim3((unsigned)a.rows), N, bytes, stream>>>(
+                     static_cast<const T*>(a.logits), a.row_stride, a.classes, a.k, inv_t,
+                     a.values, a.vtype, a.indices, a.rest, a.loss,
+                     reinterpret_cast<RowStats*>(a.stats));
+               };
+               if (once) launch(distill_fwd_kernel<T, V, N, true>);
+               else launch(distill_fwd_kernel<T, V, N, false>);
              }));
   return hipGetLastError();
 }
 
 hipError_t distill_bwd(const DistillArgs& a, hipStream_t stream) {
   // bf16: 1536 x 1000: 4.6 us by 64 threads, 4.5 by 256, 7.4 by 1024; 1024 x
-  // 16384: 13 us by 256, 15 by 64; 8192 x 32000: 212 us by 256, 178 by 1024.
+  // 16384: 13 us by 256, 15 by 64; 8192 x 32000: 212 us by 256, 178 by 1024
+  // (a copy's rate).
   const int threads = a.classes <= 1024 ? 64 : a.classes <= 16384 ? 256 : 1024;
   const float inv_t = 1.f / a.temperature;
   LOGIT_TYPE(a.type, ROW_THREADS(threads, 1024, {
@@ -784,16 +811,15 @@ hipError_t distill_bwd(const DistillArgs& a, hipStream_t stream) {
                    (reinterpret_cast<unsigned long long>(z) -
                     reinterpret_cast<unsigned long long>(grad)) % 16 == 0 &&
                    (a.row_stride - a.classes) * (long long)sizeof(T) % 16 == 0;
-               if (alike)
-                 distill_bwd_kernel<T, V, N><<<dim3((unsigned)a.rows), N, 0, stream>>>(
+               auto launch = [&](auto kernel) {
+                 kernel<<<dim3((unsigned)a.rows), N, 0, stream>>>(
                      z, a.row_stride, a.classes, a.k, inv_t, a.values, a.vtype, a.indices,
                      reinterpret_cast<const RowStats*>(a.stats), a.upstream,
                      a.upstream_stride, grad);
-               else
-                 distill_bwd_kernel<T, 1, N><<<dim3((unsigned)a.rows), N, 0, stream>>>(
-                     z, a.row_stride, a.classes, a.k, inv_t, a.values, a.vtype, a.indices,
-                     reinterpret_cast<const RowStats*>(a.stats), a.upstream,
-                     a.upstream_stride, grad);
+               };
+               if (!alike) launch(distill_bwd_kernel<T, 1, N, false>);
+               else if (past_caches(a)) launch(distill_bwd_kernel<T, V, N, true>);
+               else launch(distill_bwd_kernel<T, V, N, false>);
              }));
   return hipGetLastError();
 }
