@@ -28,27 +28,44 @@ constexpr int kBlock = 256, kGroupBlock = 512;
 constexpr int kTileRows = 4;  // rows of a tile that one thread takes
 
 struct GnPlan {
-  int vec, cpb, ctiles, chunks;
+  // Where 16 bytes do not divide the channels, `fold` rows are taken as one of
+  // c = fold * channels: a whole number of vectors. Channel i of such a row is
+  // channel i % channels of the image. Without it 23x274x152x151 bf16 (vectors
+  // of 4 bytes) takes 708 us forward and backward, and so 523.
+  int vec, fold, c;
+  long long hw;
+  int cpb, ctiles, chunks;
   int span;  // groups that a tile of channels can reach into
 };
 
 GnPlan gn_plan(const GnArgs& a) {
-  const int vec = gn_vec(a);
+  GnPlan g = {};
+  for (g.vec = 16 / gn_elem(a.type); g.vec > 1; g.vec /= 2) {
+    g.fold = g.vec / gcd_of(a.c, g.vec);
+    if (a.hw % g.fold == 0 && gn_aligned(a, g.vec)) break;
+  }
+  if (g.vec == 1) g.fold = 1;
+  g.c = a.c * g.fold;
+  g.hw = a.hw / g.fold;
   // A thread takes 16 rows at least, for a block's sums have a price: 32x336
   // x38x38 bf16 takes 36 us forward with 16, 48 with 4. Where that leaves CUs
   // without work it takes fewer: 1x480x75x75 fp16 23 us with 4, 26 with 16.
   DfdPlan p = {};
   for (int rows = 16; rows >= 4; rows /= 2) {
-    p = dfd_plan(a.c / vec, a.hw, a.n, rows);
+    p = dfd_plan(g.c / g.vec, g.hw, a.n, rows);
     if (a.n * p.chunks * p.ctiles >= 256) break;
   }
   const long long tile = kTileRows * (kBlock / p.cpb);
-  const long long tiles = (a.hw + tile - 1) / tile;
+  const long long tiles = (g.hw + tile - 1) / tile;
   long long chunks = p.chunks;
-  if (chunks < a.hw >> 20) chunks = a.hw >> 20;  // a block's rows are in div_small's range
+  if (chunks < g.hw >> 20) chunks = g.hw >> 20;  // a block's rows are in div_small's range
   if (chunks > tiles) chunks = tiles;
   const int cpg = a.c / a.groups;
-  return {vec, p.cpb, p.ctiles, (int)chunks, (p.cpb * vec + cpg - 2) / cpg + 1};
+  g.cpb = p.cpb;
+  g.ctiles = p.ctiles;
+  g.chunks = (int)chunks;
+  g.span = (p.cpb * g.vec + cpg - 2) / cpg + 1;
+  return g;
 }
 
 // Which rows and channels a thread of the streaming kernels takes. Blocks run
@@ -203,25 +220,29 @@ __global__ __launch_bounds__(kBlock) void gn_stats_kernel(
     gn_store_groups<kWave>(sum, part + (long long)blockIdx.x * span, g0, g1, cpg, first, width, each);
 }
 
-// One wave a group: joins the chunks' and tiles' moments.
+// One wave a group: joins the moments of the chunks, of the tiles that reach
+// into the group, and of the group's places in a folded row.
 __global__ __launch_bounds__(kBlock) void gn_finalize_kernel(
     const Moments* __restrict__ part, float* __restrict__ mean, float* __restrict__ rstd,
-    long long total, int cpg, int groups, int tile, int ctiles, int chunks, int span,
+    long long total, int cpg, int groups, int fold, int tile, int ctiles, int chunks, int span,
     float eps) {
   const long long id = (long long)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
   if (id >= total) return;
   const long long image = id / groups;
   const int g = (int)(id - image * groups);
-  // the tiles that reach into the group
-  const int t0 = g * cpg / tile, tiles = (g * cpg + cpg - 1) / tile - t0 + 1;
-  const float inv_tiles = 1.f / (float)tiles;
-  const Moments m = gather<kWave>(chunks * tiles, [&](int e) {
-    const int ch = div_small(e, inv_tiles), t = t0 + (e - ch * tiles);
-    return part[((image * chunks + ch) * ctiles + t) * span + (g - t * tile / cpg)];
+  const int most = (cpg + tile - 2) / tile + 1;  // tiles that can reach into a group
+  const float inv_most = 1.f / (float)most, inv_chunks = 1.f / (float)chunks;
+  const Moments m = gather<kWave>(fold * chunks * most, [&](int e) {
+    const int f = div_small(e, inv_most), place = div_small(f, inv_chunks);
+    const int ch = f - place * chunks;
+    const int from = (place * groups + g) * cpg;  // the group's first channel in the row
+    const int t = from / tile + (e - f * most);
+    if (t * tile >= from + cpg) return Moments{0.f, 0.f, 0.f};
+    return part[((image * chunks + ch) * ctiles + t) * span + (from / cpg - t * tile / cpg)];
   });
   if (threadIdx.x % kWave == 0) {
     mean[id] = m.mean;
-    rstd[id] = rsqrtf(m.m2 / m.n + eps);
+    rstd[id] = rsqrtf(m.m2 * __builtin_amdgcn_rcpf(m.n) + eps);
   }
 }
 
@@ -230,13 +251,14 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(
     const T* __restrict__ x, Params weight, Params bias,
     const T* __restrict__ residual, const float* __restrict__ drop, T* __restrict__ y,
     const float* __restrict__ mean, const float* __restrict__ rstd, long long hw, int c,
-    int groups, int cpb, int ctiles, int chunks, int turns) {
+    int groups, int cpg, int cpb, int ctiles, int chunks, int turns) {
   extern __shared__ float lds[];
   const int b = gridDim.x - 1 - blockIdx.x;
   const Place p = gn_place<VEC>(b, hw, c, cpb, ctiles, chunks, turns);
-  const float inv_cpg = 1.f / (float)(c / groups);
+  const float inv_cpg = 1.f / (float)cpg, inv_channels = 1.f / (float)(cpg * groups);
   float k[3][VEC];  // mean, factor, bias
-  gn_coefs<3, VEC>(lds, p, c, cpb, ctiles, b, [&](int ch, float (&v)[3]) {
+  gn_coefs<3, VEC>(lds, p, c, cpb, ctiles, b, [&](int i, float (&v)[3]) {
+    const int ch = i - div_small(i, inv_channels) * cpg * groups;
     const long long s = p.image * groups + div_small(ch, inv_cpg);
     v[0] = mean[s];
     v[1] = rstd[s] * weight.at(ch, 1.f);
@@ -265,13 +287,14 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, Params weight,
     Params bias, const float* __restrict__ drop,
     const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part,
-    long long hw, int c, int groups, int cpb, int ctiles, int chunks) {
+    long long hw, int c, int groups, int cpg, int cpb, int ctiles, int chunks) {
   __shared__ float l1[kBlock * VEC], l2[kBlock * VEC];
   extern __shared__ float lds[];
   const Place p = gn_place<VEC>(blockIdx.x, hw, c, cpb, ctiles, chunks, 0);
-  const float inv_cpg = 1.f / (float)(c / groups);
+  const float inv_cpg = 1.f / (float)cpg, inv_channels = 1.f / (float)(cpg * groups);
   float k[3][VEC];  // mean, factor, bias
-  gn_coefs<3, VEC>(lds, p, c, cpb, ctiles, blockIdx.x, [&](int ch, float (&v)[3]) {
+  gn_coefs<3, VEC>(lds, p, c, cpb, ctiles, blockIdx.x, [&](int i, float (&v)[3]) {
+    const int ch = i - div_small(i, inv_channels) * cpg * groups;
     const long long s = p.image * groups + div_small(ch, inv_cpg);
     v[0] = mean[s];
     v[1] = rstd[s] * weight.at(ch, 1.f);
@@ -330,28 +353,32 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(
 }
 
 // A block takes some whole groups of an image, `width` channels: their sums
-// over the chunks,
+// over the chunks and the places in a folded row,
 //   k[image][group] = (A / m, B rstd / m), so that
 //     dx = rstd (weight g - k.x - (x - mean) k.y)
 //   sums[image][2][c] = sum g, sum g h, if the parameters want them
 __global__ __launch_bounds__(kGroupBlock) void gn_bwd_group_kernel(
     const float* __restrict__ part, Params weight, const float* __restrict__ rstd,
     float2* __restrict__ k, float* __restrict__ sums, long long hw, int c, int groups,
-    int chunks, int width, int tiles) {
+    int fold, int chunks, int width, int tiles) {
   extern __shared__ float lds[];  // [2][parts * cols]
   const long long image = blockIdx.x / tiles;
   const int c0 = (int)(blockIdx.x % tiles) * width;
   const int cols = c - c0 < width ? c - c0 : width;
   const int cpg = c / groups;
   const int parts = cols < kGroupBlock ? kGroupBlock / cols : 1;
-  const float* src = part + image * chunks * 2 * c + c0;
+  // part[image][chunk][2][fold][c]
+  const float* src = part + image * chunks * 2 * fold * c + c0;
+  const float inv_fold = 1.f / (float)fold;
   for (int i = threadIdx.x; i < parts * cols; i += kGroupBlock) {
     const int p = i / cols, col = i - p * cols;
     float a = 0.f, b = 0.f;
 #pragma unroll 4
-    for (int ch = p; ch < chunks; ch += parts) {
-      a += src[(long long)ch * 2 * c + col];
-      b += src[(long long)ch * 2 * c + c + col];
+    for (int e = p; e < chunks * fold; e += parts) {
+      const int ch = div_small(e, inv_fold);
+      const float* at = src + ((long long)ch * 2 * fold + (e - ch * fold)) * c + col;
+      a += at[0];
+      b += at[(long long)fold * c];
     }
     lds[i] = a;
     lds[parts * cols + i] = b;
@@ -424,14 +451,15 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_dx_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, Params weight,
     Params bias, const float* __restrict__ drop,
     const float* __restrict__ mean, const float* __restrict__ rstd,
-    const float2* __restrict__ k, T* __restrict__ dx, long long hw, int c, int groups,
+    const float2* __restrict__ k, T* __restrict__ dx, long long hw, int c, int groups, int cpg,
     int cpb, int ctiles, int chunks, int turns) {
   extern __shared__ float lds[];
   const int b = gridDim.x - 1 - blockIdx.x;
   const Place p = gn_place<VEC>(b, hw, c, cpb, ctiles, chunks, turns);
-  const float inv_cpg = 1.f / (float)(c / groups);
+  const float inv_cpg = 1.f / (float)cpg, inv_channels = 1.f / (float)(cpg * groups);
   float q[5][VEC];  // mean, factor, bias, and what is taken off
-  gn_coefs<5, VEC>(lds, p, c, cpb, ctiles, b, [&](int ch, float (&v)[5]) {
+  gn_coefs<5, VEC>(lds, p, c, cpb, ctiles, b, [&](int i, float (&v)[5]) {
+    const int ch = i - div_small(i, inv_channels) * cpg * groups;
     const long long s = p.image * groups + div_small(ch, inv_cpg);
     const float r = rstd[s];
     const float2 kk = k[s];
@@ -469,19 +497,22 @@ long long gn_fwd_ws(const GnArgs& a) {
 // The images' sums for the parameters; streaming, the chunks' and groups' too.
 long long gn_bwd_ws(const GnArgs& a) {
   const long long sums = a.n * 2 * a.c;
-  return gn_slab_fits(a, true) ? sums : sums + a.n * gn_plan(a).chunks * a.c * 2 + a.n * a.groups * 2;
+  if (gn_slab_fits(a, true)) return sums;
+  const GnPlan p = gn_plan(a);
+  return sums + a.n * p.chunks * p.c * 2 + a.n * a.groups * 2;
 }
 
 // Tiles of a block of the kernels that make no sums: 26x256x300x300 bf16 takes
 // 407 us forward with two, 449 with one and 411 with four, for a block's
 // coefficients have a price; 4x144x150x150 14.4 with one and 16.5 with two.
 static int gn_turns(const GnArgs& a, const GnPlan& p) {
-  const long long tiles = (a.hw + kTileRows * (kBlock / p.cpb) - 1) / (kTileRows * (kBlock / p.cpb));
+  const long long tile = kTileRows * (kBlock / p.cpb);
+  const long long tiles = (p.hw + tile - 1) / tile;
   return a.n * p.ctiles * tiles >= 4096 ? 2 : 1;
 }
 static int gn_short_chunks(const GnArgs& a, const GnPlan& p) {
   const long long rows = (long long)gn_turns(a, p) * kTileRows * (kBlock / p.cpb);
-  return (int)((a.hw + rows - 1) / rows);
+  return (int)((p.hw + rows - 1) / rows);
 }
 
 hipError_t gn_fwd(const GnArgs& a, hipStream_t stream) {
@@ -500,15 +531,15 @@ hipError_t gn_fwd(const GnArgs& a, hipStream_t stream) {
   GN_TYPE(a.type, GN_VEC(p.vec, {
             const T* x = static_cast<const T*>(a.x);
             gn_stats_kernel<T, V><<<grid, kBlock, lds, stream>>>(
-                x, reinterpret_cast<Moments*>(a.ws), a.hw, a.c, cpg, p.cpb, p.ctiles,
+                x, reinterpret_cast<Moments*>(a.ws), p.hw, p.c, cpg, p.cpb, p.ctiles,
                 p.chunks, p.span);
             gn_finalize_kernel<<<waves, kBlock, 0, stream>>>(
                 reinterpret_cast<const Moments*>(a.ws), a.mean, a.rstd, groups, cpg, a.groups,
-                p.cpb * p.vec, p.ctiles, p.chunks, p.span, a.eps);
+                p.fold, p.cpb * p.vec, p.ctiles, p.chunks, p.span, a.eps);
             GN_ACT(a.act, gn_apply_kernel<T, V, A><<<fine, kBlock, coef, stream>>>(
                               x, weight, bias, static_cast<const T*>(a.residual), a.drop,
-                              static_cast<T*>(a.y), a.mean, a.rstd, a.hw, a.c, a.groups, p.cpb,
-                              p.ctiles, chunks, gn_turns(a, p)));
+                              static_cast<T*>(a.y), a.mean, a.rstd, p.hw, p.c, a.groups, cpg,
+                              p.cpb, p.ctiles, chunks, gn_turns(a, p)));
           }));
   return hipGetLastError();
 }
@@ -537,14 +568,15 @@ hipError_t gn_bwd(const GnArgs& a, hipStream_t stream) {
               const T* x = static_cast<const T*>(a.x);
               const T* dy = static_cast<const T*>(a.dy);
               gn_bwd_sums_kernel<T, V, A><<<grid, kBlock, 3 * coef, stream>>>(
-                  dy, x, weight, bias, a.drop, a.mean, a.rstd, part, a.hw, a.c, a.groups,
-                  p.cpb, p.ctiles, p.chunks);
+                  dy, x, weight, bias, a.drop, a.mean, a.rstd, part, p.hw, p.c, a.groups,
+                  cpg, p.cpb, p.ctiles, p.chunks);
               gn_bwd_group_kernel<<<dim3((unsigned)(a.n * tiles)), kGroupBlock, lds, stream>>>(
-                  part, weight, a.rstd, k, sums, a.hw, a.c, a.groups, p.chunks, width, tiles);
+                  part, weight, a.rstd, k, sums, a.hw, a.c, a.groups, p.fold, p.chunks, width,
+                  tiles);
               if (a.dx)
                 gn_bwd_dx_kernel<T, V, A><<<fine, kBlock, 5 * coef, stream>>>(
                     dy, x, weight, bias, a.drop, a.mean, a.rstd, k, static_cast<T*>(a.dx),
-                    a.hw, a.c, a.groups, p.cpb, p.ctiles, chunks, gn_turns(a, p));
+                    p.hw, p.c, a.groups, cpg, p.cpb, p.ctiles, chunks, gn_turns(a, p));
             })));
   }
   if (sums)

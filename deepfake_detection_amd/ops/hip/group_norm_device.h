@@ -381,12 +381,18 @@ DFD_DEV void gn_store_once(T* p, const DfdVec<T, VEC>& x) {
 // and that every tensor's address allows.
 static inline int gn_elem(GnType t) { return t == GnType::kF32 ? 4 : 2; }
 
-static inline int gn_vec(const GnArgs& a) {
-  const int es = gn_elem(a.type);
-  int vec = dfd_pick_vec(a.c, es);
+static inline int gcd_of(int a, int b) { return b ? gcd_of(b, a % b) : a; }
+
+static inline bool gn_aligned(const GnArgs& a, int vec) {
   const void* ptrs[] = {a.x, a.y, a.residual, a.dy, a.dx};
   for (const void* p : ptrs)
-    while (vec > 1 && reinterpret_cast<unsigned long long>(p) % (vec * es) != 0) vec >>= 1;
+    if (reinterpret_cast<unsigned long long>(p) % (vec * gn_elem(a.type)) != 0) return false;
+  return true;
+}
+
+static inline int gn_vec(const GnArgs& a) {
+  int vec = dfd_pick_vec(a.c, gn_elem(a.type));
+  while (vec > 1 && !gn_aligned(a, vec)) vec >>= 1;
   return vec;
 }
 

@@ -30,8 +30,6 @@ struct SlabPlan {
   int lds;
 };
 
-int gcd_of(int a, int b) { return b ? gcd_of(b, a % b) : a; }
-
 bool slab_try(const GnArgs& a, int tensors, int vec, int width, int threads, SlabPlan* p) {
   const int cpg = a.c / a.groups;
   p->vec = vec;

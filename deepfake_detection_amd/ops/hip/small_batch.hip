@@ -258,7 +258,7 @@ at::Tensor group_norm_act(at::Tensor x, OptTensor weight_opt,
   TORCH_CHECK(x.is_cuda() && x.dim() == 4, who, ": 4D CUDA tensor expected");
   gn_type(x, who);
   const int64_t c = x.size(1);
-  TORCH_CHECK(c <= 1 << 20, who, ": more than 2^20 channels");
+  TORCH_CHECK(c <= 1 << 18, who, ": more than 2^18 channels");
   TORCH_CHECK(groups > 0 && c % groups == 0, who, ": ", c, " channels are not a multiple of ",
               groups, " groups");
   Act act = Act::kNone;

@@ -37,6 +37,11 @@ SHAPES = [
     (1, 16400, 16, 2, 3),
     (66, 32, 4, 48, 48),   # bf16: a slab of nearly all of a block's LDS
     (3, 4, 4, 1, 1),       # one value a group
+    (2, 274, 2, 60, 62),   # widths that 16 bytes do not divide: rows are folded
+    (1, 33, 1, 120, 136),
+    (2, 150, 6, 90, 98),
+    (3, 11, 1, 130, 176),
+    (1, 50, 5, 151, 149),  # and an odd number of rows, which cannot be
     (1, 16, 4, 270, 260),  # more rows than a slab's indexes take
 ]
 
