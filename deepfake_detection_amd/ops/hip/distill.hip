@@ -745,7 +745,7 @@ static void topk_launch(const TopkArgs& a, hipStream_t stream) {
         z, a.row_stride, a.classes, a.k, inv_t, values, a.indices, a.rest);
 }
 
-hipError_t topk_logits_launch(const TopkArgs& a, hipStream_t stream) {
+static hipError_t topk_rows(const TopkArgs& a, hipStream_t stream) {
   // A wave alone has no barriers to wait at, and many rows hide its own time;
   // more threads shorten a row's. us by 64, 256 and 512 threads: bf16, k = 16,
   // 4096 x 16000: 36, 44, 59; 4096 x 32000: 63, 65, 76; fp16, k = 12, 4929 x
@@ -774,7 +774,7 @@ static bool past_caches(const DistillArgs& a) {
   return a.rows * a.classes * (a.type == LogitType::kF32 ? 4 : 2) > 256ll << 20;
 }
 
-hipError_t distill_fwd(const DistillArgs& a, hipStream_t stream) {
+static hipError_t fwd_rows(const DistillArgs& a, hipStream_t stream) {
   // bf16: 1536 x 2048: 10.5 us by 64 threads, 11.4 by 256; 8192 x 32000 (all
   // through the cache): 147 us by 256, 170 by 64; 32 x 131072: 24 us by 256, 18
   // by 512, 17 by 1024.
@@ -796,7 +796,7 @@ hipError_t distill_fwd(const DistillArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t distill_bwd(const DistillArgs& a, hipStream_t stream) {
+static hipError_t bwd_rows(const DistillArgs& a, hipStream_t stream) {
   // bf16: 1536 x 1000: 4.6 us by 64 threads, 4.5 by 256, 7.4 by 1024; 1024 x
   // 16384: 13 us by 256, 15 by 64; 8192 x 32000: 212 us by 256, 178 by 1024
   // (a copy's rate).
@@ -822,4 +822,58 @@ hipError_t distill_bwd(const DistillArgs& a, hipStream_t stream) {
                else launch(distill_bwd_kernel<T, V, N, false>);
              }));
   return hipGetLastError();
+}
+
+// HIP takes fewer than 2^32 threads a launch: more rows go in several.
+constexpr long long kMostRows = 1ll << 21;
+
+static const void* at(const void* p, LogitType type, long long i) {
+  return static_cast<const char*>(p) + i * (type == LogitType::kF32 ? 4 : 2);
+}
+static void* at(void* p, LogitType type, long long i) {
+  return static_cast<char*>(p) + i * (type == LogitType::kF32 ? 4 : 2);
+}
+
+// f of the args of each part of the rows.
+template <typename Args, typename Skip, typename F>
+static hipError_t in_parts(const Args& all, Skip skip, F f) {
+  Args a = all;
+  hipError_t e = hipSuccess;
+  for (long long left = all.rows; left > 0 && e == hipSuccess; left -= a.rows) {
+    a.rows = left < kMostRows ? left : kMostRows;
+    e = f(a);
+    skip(a, a.rows);
+  }
+  return e;
+}
+
+hipError_t topk_logits_launch(const TopkArgs& args, hipStream_t stream) {
+  return in_parts(
+      args,
+      [](TopkArgs& a, long long n) {
+        a.logits = at(a.logits, a.type, n * a.row_stride);
+        a.values = at(a.values, a.type, n * a.k);
+        a.indices += n * a.k;
+        a.rest += n;
+      },
+      [&](const TopkArgs& a) { return topk_rows(a, stream); });
+}
+
+static void distill_skip(DistillArgs& a, long long n) {
+  a.logits = at(a.logits, a.type, n * a.row_stride);
+  a.values = at(a.values, a.vtype, n * a.k);
+  a.indices += n * a.k;
+  a.stats += n * kDistillStats;
+  if (a.rest) a.rest += n;
+  if (a.loss) a.loss += n;
+  if (a.upstream) a.upstream += n * a.upstream_stride;
+  if (a.grad) a.grad = at(a.grad, a.type, n * a.classes);
+}
+
+hipError_t distill_fwd(const DistillArgs& args, hipStream_t stream) {
+  return in_parts(args, distill_skip, [&](const DistillArgs& a) { return fwd_rows(a, stream); });
+}
+
+hipError_t distill_bwd(const DistillArgs& args, hipStream_t stream) {
+  return in_parts(args, distill_skip, [&](const DistillArgs& a) { return bwd_rows(a, stream); });
 }

@@ -457,6 +457,32 @@ def test_rows_beyond_32_bits():
         assert torch.equal(grad[i], grad[0])
 
 
+@pytest.mark.gpu
+def test_more_rows_than_one_launch():
+    """Rows beyond 2^21 go in a launch of their own: their results are those of
+    the rows alone."""
+    rows, classes, k = 2 ** 21 + 5, 3, 2
+    g = torch.Generator(device="cuda").manual_seed(5)
+    wide = torch.randn(rows, classes + 1, device="cuda", generator=g)
+    z, teacher = wide[:, :classes], torch.randn(rows, classes, device="cuda", generator=g)
+    up = torch.rand(rows, device="cuda", generator=g)
+    answer = O.topk_logits(teacher, k, 2.0)
+
+    def run(z, answer, up):
+        leaf = z.detach().requires_grad_()
+        loss = O.distill_topk(leaf, *answer, temperature=2.0)
+        return loss, torch.autograd.grad(loss, leaf, up)[0]
+
+    loss, grad = run(z, answer, up)
+    for part in (slice(0, 100), slice(2 ** 21 - 3, rows)):
+        for got, want in zip(answer, O.topk_logits(teacher[part], k, 2.0)):
+            assert torch.equal(got[part], want)
+        want = run(z[part], [a[part] for a in answer], up[part])
+        assert torch.equal(loss[part], want[0]) and torch.equal(grad[part], want[1])
+    assert torch.equal(answer[0][:, 0], teacher.amax(1))
+    assert torch.isfinite(loss).all() and (loss >= 0).all()
+
+
 def training_step(z, teacher, k, t):
     answer = O.topk_logits(teacher, k, t)
     leaf = z.detach().requires_grad_()
