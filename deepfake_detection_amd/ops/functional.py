@@ -136,8 +136,8 @@ def group_norm_act(x, gn, act: str = "silu", residual=None, drop_path_mask=None)
     other images change an image's result, in training and in eval alike.
     GPU: HIP kernels (ops/hip/group_norm.hip), channels_last in and out (other
     layouts are copied), fp32/bf16/fp16, statistics and parameter gradients in
-    fp32; differentiable once, in x, the parameters and residual. CPU: torch
-    ops of the same result.
+    fp32; differentiable once, in x, the parameters and residual; at most 2^18
+    channels, 2^14 in a group. CPU: torch ops of the same result.
 
     gn: an ``nn.GroupNorm`` (its num_groups, eps, weight and bias are used).
     act: "silu", "relu" or "none". drop_path_mask: [B] per-sample 0-or-1/keep
@@ -219,8 +219,9 @@ def distill_topk(logits, values, indices, rest=None, temperature: float = 1.0):
     finite rest teaches nothing: its loss and gradient are 0, whatever its
     logits hold. An index beyond the classes makes its row's loss and gradient
     NaN. If two slots name one class, each has its own term in the loss and their
-    probabilities add up in the gradient. A class at -inf has student probability 0; where the teacher gives it more, the loss
-    is inf. The loss is not scaled by temperature^2. Differentiable once, in
+    probabilities add up in the gradient. A class at -inf has student probability
+    0; where the teacher gives it more, the loss is inf. The loss is not scaled
+    by temperature^2. Differentiable once, in
     logits; the teacher's answer is given. GPU: one pass over the logits
     forward, one backward (ops/hip/distill.hip).
     """

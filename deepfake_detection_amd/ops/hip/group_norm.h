@@ -1,6 +1,7 @@
 // Launchers of the group norm + activation kernels (group_norm.hip). Raw
 // pointers only: shapes, types, devices and layouts are checked by the caller
-// (small_batch.hip).
+// (small_batch.hip). A launch of 2^32 threads or more, which HIP does not take,
+// is hipErrorInvalidConfiguration, before anything has run.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -10,6 +11,8 @@ enum class GnType : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 // x, y, residual, dy, dx: [n, hw, c] row-major (channels last), one type.
 // weight, bias: [c] of type ptype, or null. mean, rstd: fp32 [n, groups].
 // drop: fp32 [n] or null.
+constexpr int kGnMaxGroupChannels = 1 << 14;  // their sums are joined in LDS
+
 struct GnArgs {
   long long n, hw;
   int c, groups;
@@ -39,7 +42,7 @@ long long gn_bwd_ws(const GnArgs& a);
 hipError_t gn_fwd(const GnArgs& a, hipStream_t stream);
 hipError_t gn_bwd(const GnArgs& a, hipStream_t stream);
 
-// Slabs in registers (group_norm_slab.hip). sums: [n, 2, c] floats, the images'
+// Slabs held in LDS (group_norm_slab.hip). sums: [n, 2, c] floats, the images'
 // parts of dbias and dweight, or null.
 bool gn_slab_fits(const GnArgs& a, bool backward);
 hipError_t gn_slab_fwd(const GnArgs& a, hipStream_t stream);

@@ -31,7 +31,7 @@ struct GnPlan {
   // Where 16 bytes do not divide the channels, `fold` rows are taken as one of
   // c = fold * channels: a whole number of vectors. Channel i of such a row is
   // channel i % channels of the image. Without it 23x274x152x151 bf16 (vectors
-  // of 4 bytes) takes 708 us forward and backward, and so 523.
+  // of 4 bytes) takes 702 us forward and backward, and so 513.
   int vec, fold, c;
   long long hw;
   int cpb, ctiles, chunks;
@@ -48,8 +48,9 @@ GnPlan gn_plan(const GnArgs& a) {
   g.c = a.c * g.fold;
   g.hw = a.hw / g.fold;
   // A thread takes 16 rows at least, for a block's sums have a price: 32x336
-  // x38x38 bf16 takes 36 us forward with 16, 48 with 4. Where that leaves CUs
-  // without work it takes fewer: 1x480x75x75 fp16 23 us with 4, 26 with 16.
+  // x38x38 bf16 takes 32 us forward and 48 backward with 16, 37 and 53 with 4.
+  // Where that leaves CUs without work it takes fewer: 1x480x75x75 fp16 26 and
+  // 27 with 4, 21 and 34 with 16.
   DfdPlan p = {};
   for (int rows = 16; rows >= 4; rows /= 2) {
     p = dfd_plan(g.c / g.vec, g.hw, a.n, rows);
@@ -416,17 +417,20 @@ __global__ __launch_bounds__(kGroupBlock) void gn_bwd_group_kernel(
 }
 
 // dbias[c], dweight[c] from the images' sums: 32 channels a block, 32 threads
-// for each of them.
+// for each of them. Slice blockIdx.y takes `per` images; its result is 2 c
+// after the one before.
 __global__ __launch_bounds__(1024) void gn_bwd_params_kernel(
     const float* __restrict__ sums, float* __restrict__ dweight, float* __restrict__ dbias,
-    long long n, int c) {
+    long long n, int c, int per) {
   __shared__ float l1[1024], l2[1024];
   const int t = threadIdx.x;
   const int ch = blockIdx.x * 32 + t % 32;
+  const long long first = (long long)blockIdx.y * per;
+  const long long end = first + per < n ? first + per : n;
   float s1 = 0.f, s2 = 0.f;
   if (ch < c) {
 #pragma unroll 4
-    for (long long i = t / 32; i < n; i += 32) {
+    for (long long i = first + t / 32; i < end; i += 32) {
       s1 += sums[i * 2 * c + ch];
       s2 += sums[i * 2 * c + c + ch];
     }
@@ -441,8 +445,8 @@ __global__ __launch_bounds__(1024) void gn_bwd_params_kernel(
     }
   }
   if (t < 32 && ch < c) {
-    if (dbias) dbias[ch] = l1[t];
-    if (dweight) dweight[ch] = l2[t];
+    if (dbias) dbias[blockIdx.y * 2ll * c + ch] = l1[t];
+    if (dweight) dweight[blockIdx.y * 2ll * c + ch] = l2[t];
   }
 }
 
@@ -494,9 +498,19 @@ long long gn_fwd_ws(const GnArgs& a) {
   return a.n * p.chunks * p.ctiles * p.span * (long long)(sizeof(Moments) / sizeof(float));
 }
 
-// The images' sums for the parameters; streaming, the chunks' and groups' too.
+// Images that one block of the parameters' kernel adds up; where there are
+// more, the slices' results are added in a second launch: backward of 16384x256
+// x1x1 bf16 49 us so and 105 by one launch, 4096x448x3x3 61 and 68.
+static int gn_slice(const GnArgs& a) {
+  const long long per = a.n <= 512 ? a.n : a.n <= 64 * 256 ? 256 : (a.n + 63) / 64;
+  return (int)per;
+}
+static int gn_slices(const GnArgs& a) { return (int)((a.n + gn_slice(a) - 1) / gn_slice(a)); }
+
+// The images' sums for the parameters, and the slices'; streaming, the chunks'
+// and groups' too.
 long long gn_bwd_ws(const GnArgs& a) {
-  const long long sums = a.n * 2 * a.c;
+  const long long sums = (a.n + gn_slices(a)) * 2 * a.c;
   if (gn_slab_fits(a, true)) return sums;
   const GnPlan p = gn_plan(a);
   return sums + a.n * p.chunks * p.c * 2 + a.n * a.groups * 2;
@@ -519,6 +533,9 @@ hipError_t gn_fwd(const GnArgs& a, hipStream_t stream) {
   if (gn_slab_fits(a, false)) return gn_slab_fwd(a, stream);
   const GnPlan p = gn_plan(a);
   const int chunks = gn_short_chunks(a, p);
+  if (gn_too_many(a.n * chunks * p.ctiles, kBlock) ||
+      gn_too_many((a.n * a.groups + 3) / 4, kBlock))
+    return hipErrorInvalidConfiguration;
   const dim3 fine((unsigned)(a.n * chunks * p.ctiles));
   const int coef = 3 * (int)sizeof(float) * p.cpb * p.vec;
   const Params weight = {a.weight, a.ptype}, bias = {a.bias, a.ptype};
@@ -556,14 +573,16 @@ hipError_t gn_bwd(const GnArgs& a, hipStream_t stream) {
     const int chunks = gn_short_chunks(a, p);
     const dim3 fine((unsigned)(a.n * chunks * p.ctiles));
     const int coef = (int)sizeof(float) * p.cpb * p.vec;  // LDS of one coefficient
-    float2* k = reinterpret_cast<float2*>(a.ws + a.n * 2 * a.c);
-    float* part = a.ws + a.n * 2 * a.c + a.n * a.groups * 2;
+    float2* k = reinterpret_cast<float2*>(a.ws + (a.n + gn_slices(a)) * 2 * a.c);
+    float* part = reinterpret_cast<float*>(k + a.n * a.groups);
     // whole groups of about 32 channels: many blocks, and many threads a
     // channel, since the chunks are read one after another
     const int cpg = a.c / a.groups;
     const int width = cpg >= 32 ? cpg : 32 / cpg * cpg;
     const int tiles = (a.c + width - 1) / width;
     const int lds = 2 * (int)sizeof(float) * (width > kGroupBlock ? width : kGroupBlock);
+    if (gn_too_many(a.n * chunks * p.ctiles, kBlock) || gn_too_many(a.n * tiles, kGroupBlock))
+      return hipErrorInvalidConfiguration;
     GN_TYPE(a.type, GN_VEC(p.vec, GN_ACT(a.act, {
               const T* x = static_cast<const T*>(a.x);
               const T* dy = static_cast<const T*>(a.dy);
@@ -579,8 +598,19 @@ hipError_t gn_bwd(const GnArgs& a, hipStream_t stream) {
                     p.hw, p.c, a.groups, cpg, p.cpb, p.ctiles, chunks, gn_turns(a, p));
             })));
   }
-  if (sums)
-    gn_bwd_params_kernel<<<dim3((a.c + 31) / 32), 1024, 0, stream>>>(sums, a.dweight, a.dbias,
-                                                                     a.n, a.c);
+  if (sums) {
+    const unsigned blocks = (a.c + 31) / 32;
+    const int slices = gn_slices(a);
+    long long n = a.n;
+    if (slices > 1) {
+      float* parts = a.ws + a.n * 2 * a.c;
+      gn_bwd_params_kernel<<<dim3(blocks, slices), 1024, 0, stream>>>(
+          sums, parts + a.c, parts, n, a.c, gn_slice(a));
+      sums = parts;
+      n = slices;
+    }
+    gn_bwd_params_kernel<<<dim3(blocks), 1024, 0, stream>>>(sums, a.dweight, a.dbias, n, a.c,
+                                                            (int)n);
+  }
   return hipGetLastError();
 }

@@ -381,6 +381,10 @@ DFD_DEV void gn_store_once(T* p, const DfdVec<T, VEC>& x) {
 // and that every tensor's address allows.
 static inline int gn_elem(GnType t) { return t == GnType::kF32 ? 4 : 2; }
 
+static inline bool gn_too_many(long long blocks, int threads) {
+  return blocks * threads >= 1ll << 32;
+}
+
 static inline int gcd_of(int a, int b) { return b ? gcd_of(b, a % b) : a; }
 
 static inline bool gn_aligned(const GnArgs& a, int vec) {

@@ -11,8 +11,9 @@
 // These are small shapes, where a launch's fixed costs count: the loops stay
 // rolled, since code that runs once costs more to fetch than to run. Forward,
 // 64x160x19x19 bf16 takes 12.0 us (two passes over rows in registers, all
-// unrolled: 17.4; streaming: 38 in three launches), 32x256x19x19 fp16 9.0 (its
-// 12 MB at the rate of a large copy: 2.4), 1x1632x10x10 fp16 7.6. What is left
+// unrolled: 17.4; streaming: 17.9 in three launches), 32x256x19x19 fp16 9.0 (its
+// 12 MB at the rate of a large copy: 1.9; streaming 16.7), 1x1632x10x10 fp16 7.3
+// (streaming 13.8); backward 15.9 and 12.8 (streaming 25.8 and 24.6). What is left
 // is a block's chain: by a clock in the kernel 2.3 to 3.7 us until the rows are
 // there, 2.3 for the sums, 1.0 to 2.6 for the activation and its stores.
 
@@ -56,21 +57,29 @@ SlabPlan slab_plan(const GnArgs& a, int tensors) {
   const int widest = gn_vec(a);
   for (int vec = widest; vec >= 1; vec >>= 1) {
     // Loads of less than 8 bytes are for small tensors, where time is a
-    // launch's: 32x336x38x38 bf16 by vectors of 2 takes 37 us forward and 59
-    // backward, streaming 33 and 53.
+    // launch's: 32x336x38x38 bf16 (groups of 21 channels) by vectors of 2 takes
+    // 30 us forward and 67 backward, streaming 32 and 48.
     if (vec < widest && vec * es < 8 && a.n * a.hw * a.c * es > (4 << 20)) break;
     const int unit = cpg / gcd_of(cpg, vec) * vec;
-    // A row's part of a slab is 64 bytes or more, or 32 where it then fits.
+    // A row's part of a slab is 64 bytes or more, or 32 where it then fits. Of
+    // many images of few rows a slab is 2 KB or more: a block has its own price.
     int m = 1;
-    while (m * unit < a.c && m * unit * es < 64) ++m;
+    while (m * unit < a.c &&
+           (m * unit * es < 64 ||
+            (m * unit * es * a.hw < 2048 && a.n * a.c / (m * unit) > 4096)))
+      ++m;
     for (; m >= 1; m /= 2) {
       const int width = m * unit < a.c ? m * unit : a.c;
       const long long blocks = a.n * ((a.c + width - 1) / width);
       const bool few = blocks < 128;
       if (width * es < 32 && width < a.c && !few) break;
-      // 512x448x10x10 slabs of 13 KB: 12.7 us by 256 threads, 13.6 by 512;
-      // 256 of 29 KB: 14.5 us by 512, 15.9 by 1024; 28 of 80 KB: 13.9 us by 1024.
-      const int threads = blocks <= 64 ? 1024 : a.hw * width * es <= 16384 ? 256 : 512;
+      // 512 slabs of 13 KB: 12.7 us by 256 threads, 13.6 by 512; 256 of 29 KB:
+      // 14.5 us by 512, 15.9 by 1024; 28 of 80 KB: 13.9 us by 1024; 8192 of
+      // 3 KB (1024x256x7x7 bf16): 20.8 us by 64, 24.6 by 128, 36.8 by 256;
+      // 16384x256x1x1 bf16: 31 us by 64 in slabs of 512 bytes, 435 by 256 in
+      // slabs of 64.
+      const long long bytes = a.hw * width * es;
+      const int threads = blocks <= 64 ? 1024 : bytes <= 4096 ? 64 : bytes <= 16384 ? 256 : 512;
       if (!slab_try(a, tensors, vec, width, threads, &p)) continue;
       // With less than a block for every other CU, narrower vectors make more
       // and smaller slabs.
@@ -291,6 +300,7 @@ bool gn_slab_fits(const GnArgs& a, bool backward) {
 
 hipError_t gn_slab_fwd(const GnArgs& a, hipStream_t stream) {
   const SlabPlan p = slab_plan(a, 1);
+  if (gn_too_many(a.n * p.slices, p.threads)) return hipErrorInvalidConfiguration;
   const Params weight = {a.weight, a.ptype}, bias = {a.bias, a.ptype};
   const dim3 grid((unsigned)(a.n * p.slices));
   GN_TYPE(a.type, GN_VEC(p.vec, GN_ACT(a.act, {
@@ -304,6 +314,7 @@ hipError_t gn_slab_fwd(const GnArgs& a, hipStream_t stream) {
 
 hipError_t gn_slab_bwd(const GnArgs& a, float* sums, hipStream_t stream) {
   const SlabPlan p = slab_plan(a, 2);
+  if (gn_too_many(a.n * p.slices, p.threads)) return hipErrorInvalidConfiguration;
   const Params weight = {a.weight, a.ptype}, bias = {a.bias, a.ptype};
   const dim3 grid((unsigned)(a.n * p.slices));
   GN_TYPE(a.type, GN_VEC(p.vec, GN_ACT(a.act, {

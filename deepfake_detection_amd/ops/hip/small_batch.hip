@@ -30,6 +30,7 @@ GnType gn_type(const at::Tensor& x, const char* who) {
 }
 
 void check_launch(hipError_t e, const char* who) {
+  TORCH_CHECK(e != hipErrorInvalidConfiguration, who, ": too large for one launch");
   TORCH_CHECK(e == hipSuccess, who, ": ", hipGetErrorString(e));
 }
 
@@ -261,6 +262,7 @@ at::Tensor group_norm_act(at::Tensor x, OptTensor weight_opt,
   TORCH_CHECK(c <= 1 << 18, who, ": more than 2^18 channels");
   TORCH_CHECK(groups > 0 && c % groups == 0, who, ": ", c, " channels are not a multiple of ",
               groups, " groups");
+  TORCH_CHECK(c / groups <= kGnMaxGroupChannels, who, ": more than 2^14 channels in a group");
   Act act = Act::kNone;
   if (act_s == "relu") act = Act::kRelu;
   else if (act_s == "silu") act = Act::kSilu;

@@ -306,6 +306,37 @@ def test_tail_against_formulas(shape, dtype):
     against_formulas(shape, TYPES[dtype], "cuda", "silu", tail=True, affine=False)
 
 
+# many images of few rows: slabs of few threads, and the parameters' gradients
+# in slices of images
+MANY = [
+    (2100, 256, 32, 1, 2),
+    (1030, 256, 32, 7, 7),
+    (513, 48, 16, 2, 3),   # one image in the last slice
+    (600, 36, 4, 3, 1),
+    (17000, 8, 1, 1, 1),   # more slices than 64 of 256 images
+    (512, 40, 8, 5, 1),
+    (520, 64, 2, 52, 50),  # and with streaming
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_many_images(shape, dtype):
+    against_formulas(shape, TYPES[dtype], "cuda", "silu", tail=True)
+
+
+@pytest.mark.gpu
+def test_too_large_is_refused():
+    gn = nn.GroupNorm(1, 40960).cuda()
+    with pytest.raises(RuntimeError, match="channels in a group"):
+        O.group_norm_act(torch.zeros(1, 40960, 1, 1, device="cuda"), gn, "none")
+    gn = nn.GroupNorm(4, 8).cuda()
+    x = torch.zeros(2 ** 26, 8, 1, 1, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="too large for one launch"):
+        O.group_norm_act(x, gn, "none")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [SHAPES[7], SHAPES[9], SHAPES[4]], ids=str)
 def test_large_common_offset(shape):
