@@ -451,7 +451,12 @@ def test_rows_beyond_32_bits():
     z.requires_grad_()
     answer = [a.expand(rows, *a.shape[1:]) for a in answer]
     loss = O.distill_topk(z, *answer)
-    assert torch.equal(loss, want.expand(rows))
+    assert torch.equal(loss, loss[:1].expand(rows))
+    # A row alone is summed by other threads: at least 256 of them, 1024 values
+    # each one after another and eight steps to join, so either sum is within
+    # 1032 roundings of 2^-24, the loss moves by at most as much as their
+    # logarithms do, and the steps after them are the same
+    assert (loss[0] - want[0]).abs() <= 2 * 1040 * 2.0 ** -24
     (grad,) = torch.autograd.grad(loss, z, torch.ones_like(loss))
     for i in (1, rows - 1):
         assert torch.equal(grad[i], grad[0])
