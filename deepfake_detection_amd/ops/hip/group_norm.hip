@@ -117,6 +117,18 @@ DFD_DEV Place gn_place(int b, long long hw, int c, int cpb, int ctiles, int chun
   return p;
 }
 
+// Blocks go to the 8 XCDs in turn. Those that take the same rows, other
+// channels, are given the same XCD, one after another: where a tile's part of a
+// row does not end with a cache line, they share it in one L2. 20x1032x84x83
+// fp16 takes 182 us forward and 302 backward so, 212 and 332 otherwise; 26x960
+// x75x75 bf16, whose tiles do end with lines, 155 and 268, and 159 and 275.
+DFD_DEV int gn_near(int b, int ctiles) {
+  const int set = 8 * ctiles;
+  if (ctiles == 1 || b >= (int)gridDim.x / set * set) return b;
+  const int r = b % set;
+  return b - r + r % 8 * ctiles + r / 8;
+}
+
 // Per-channel coefficients of a block's channels, made once in LDS and read
 // from there into registers: coef(channel, k) for the k-th of K.
 template <int K, int VEC, typename F>
@@ -181,8 +193,9 @@ __global__ __launch_bounds__(kBlock) void gn_stats_kernel(
     const T* __restrict__ x, Moments* __restrict__ part, long long hw, int c, int cpg, int cpb,
     int ctiles, int chunks, int span) {
   extern __shared__ float lds[];
-  const Place p = gn_place<VEC>(blockIdx.x, hw, c, cpb, ctiles, chunks, 0);
-  const int first = blockIdx.x % ctiles * cpb * VEC;  // the tile's channels
+  const int b = gn_near(blockIdx.x, ctiles);
+  const Place p = gn_place<VEC>(b, hw, c, cpb, ctiles, chunks, 0);
+  const int first = b % ctiles * cpb * VEC;  // the tile's channels
   const int width = c - first < cpb * VEC ? c - first : cpb * VEC;
   // a vector within one group is one column
   const bool whole = cpg % VEC == 0;
@@ -216,9 +229,9 @@ __global__ __launch_bounds__(kBlock) void gn_stats_kernel(
   sum.join_rows(here, each);
   const int g0 = first / cpg, g1 = (first + width - 1) / cpg;
   if (sum.small_groups(g1 - g0 + 1))
-    gn_store_groups<16>(sum, part + (long long)blockIdx.x * span, g0, g1, cpg, first, width, each);
+    gn_store_groups<16>(sum, part + (long long)b * span, g0, g1, cpg, first, width, each);
   else
-    gn_store_groups<kWave>(sum, part + (long long)blockIdx.x * span, g0, g1, cpg, first, width, each);
+    gn_store_groups<kWave>(sum, part + (long long)b * span, g0, g1, cpg, first, width, each);
 }
 
 // One wave a group: joins the moments of the chunks, of the tiles that reach
@@ -254,7 +267,7 @@ __global__ __launch_bounds__(kBlock) void gn_apply_kernel(
     const float* __restrict__ mean, const float* __restrict__ rstd, long long hw, int c,
     int groups, int cpg, int cpb, int ctiles, int chunks, int turns) {
   extern __shared__ float lds[];
-  const int b = gridDim.x - 1 - blockIdx.x;
+  const int b = gn_near(gridDim.x - 1 - blockIdx.x, ctiles);
   const Place p = gn_place<VEC>(b, hw, c, cpb, ctiles, chunks, turns);
   const float inv_cpg = 1.f / (float)cpg, inv_channels = 1.f / (float)(cpg * groups);
   float k[3][VEC];  // mean, factor, bias
@@ -291,10 +304,11 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(
     long long hw, int c, int groups, int cpg, int cpb, int ctiles, int chunks) {
   __shared__ float l1[kBlock * VEC], l2[kBlock * VEC];
   extern __shared__ float lds[];
-  const Place p = gn_place<VEC>(blockIdx.x, hw, c, cpb, ctiles, chunks, 0);
+  const int b = gn_near(blockIdx.x, ctiles);
+  const Place p = gn_place<VEC>(b, hw, c, cpb, ctiles, chunks, 0);
   const float inv_cpg = 1.f / (float)cpg, inv_channels = 1.f / (float)(cpg * groups);
   float k[3][VEC];  // mean, factor, bias
-  gn_coefs<3, VEC>(lds, p, c, cpb, ctiles, blockIdx.x, [&](int i, float (&v)[3]) {
+  gn_coefs<3, VEC>(lds, p, c, cpb, ctiles, b, [&](int i, float (&v)[3]) {
     const int ch = i - div_small(i, inv_channels) * cpg * groups;
     const long long s = p.image * groups + div_small(ch, inv_cpg);
     v[0] = mean[s];
@@ -343,7 +357,7 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_sums_kernel(
     s = h;
   }
   if (p.in && p.rg == 0) {
-    const long long chunk = blockIdx.x / ctiles;
+    const long long chunk = b / ctiles;
     float* out = part + chunk * 2 * c + p.c0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -458,7 +472,7 @@ __global__ __launch_bounds__(kBlock) void gn_bwd_dx_kernel(
     const float2* __restrict__ k, T* __restrict__ dx, long long hw, int c, int groups, int cpg,
     int cpb, int ctiles, int chunks, int turns) {
   extern __shared__ float lds[];
-  const int b = gridDim.x - 1 - blockIdx.x;
+  const int b = gn_near(gridDim.x - 1 - blockIdx.x, ctiles);
   const Place p = gn_place<VEC>(b, hw, c, cpb, ctiles, chunks, turns);
   const float inv_cpg = 1.f / (float)cpg, inv_channels = 1.f / (float)(cpg * groups);
   float q[5][VEC];  // mean, factor, bias, and what is taken off
