@@ -24,7 +24,7 @@
 
 namespace {
 
-constexpr int kBlock = 256, kGroupBlock = 512;
+constexpr int kBlock = 256, kGroupBlock = 1024;  // most threads of gn_bwd_group
 constexpr int kTileRows = 4;  // rows of a tile that one thread takes
 
 struct GnPlan {
@@ -234,19 +234,31 @@ __global__ __launch_bounds__(kBlock) void gn_stats_kernel(
     gn_store_groups<kWave>(sum, part + (long long)b * span, g0, g1, cpg, first, width, each);
 }
 
-// One wave a group: joins the moments of the chunks, of the tiles that reach
+// A group's WAVES waves join the moments of the chunks, of the tiles that reach
 // into the group, and of the group's places in a folded row.
-__global__ __launch_bounds__(kBlock) void gn_finalize_kernel(
+template <int WAVES>
+constexpr int final_block() {
+  return WAVES > 1 ? WAVES * kWave : kBlock;
+}
+
+template <int WAVES>
+__global__ __launch_bounds__(final_block<WAVES>()) void gn_finalize_kernel(
     const Moments* __restrict__ part, float* __restrict__ mean, float* __restrict__ rstd,
     long long total, int cpg, int groups, int fold, int tile, int ctiles, int chunks, int span,
     float eps) {
-  const long long id = (long long)blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
-  if (id >= total) return;
+  __shared__ Moments joined[WAVES];
+  const int lanes = WAVES * kWave;
+  const long long id = (long long)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+  if (id >= total) return;  // the whole block, where a group has more than one wave
   const long long image = id / groups;
   const int g = (int)(id - image * groups);
   const int most = (cpg + tile - 2) / tile + 1;  // tiles that can reach into a group
   const float inv_most = 1.f / (float)most, inv_chunks = 1.f / (float)chunks;
-  const Moments m = gather<kWave>(fold * chunks * most, [&](int e) {
+  const int wave = threadIdx.x % lanes / kWave;
+  const int all = fold * chunks * most, each = (all + WAVES - 1) / WAVES;
+  const int begin = wave * each, count = all - begin < each ? all - begin : each;
+  Moments m = gather<kWave>(count, [&](int i) {
+    const int e = begin + i;
     const int f = div_small(e, inv_most), place = div_small(f, inv_chunks);
     const int ch = f - place * chunks;
     const int from = (place * groups + g) * cpg;  // the group's first channel in the row
@@ -254,7 +266,12 @@ __global__ __launch_bounds__(kBlock) void gn_finalize_kernel(
     if (t * tile >= from + cpg) return Moments{0.f, 0.f, 0.f};
     return part[((image * chunks + ch) * ctiles + t) * span + (from / cpg - t * tile / cpg)];
   });
-  if (threadIdx.x % kWave == 0) {
+  if (WAVES > 1) {
+    if (threadIdx.x % kWave == 0) joined[wave] = m;
+    __syncthreads();
+    m = gather<16>(WAVES, [&](int e) { return joined[e]; });
+  }
+  if (threadIdx.x % lanes == 0) {
     mean[id] = m.mean;
     rstd[id] = rsqrtf(m.m2 * __builtin_amdgcn_rcpf(m.n) + eps);
   }
@@ -376,19 +393,20 @@ __global__ __launch_bounds__(kGroupBlock) void gn_bwd_group_kernel(
     const float* __restrict__ part, Params weight, const float* __restrict__ rstd,
     float2* __restrict__ k, float* __restrict__ sums, long long hw, int c, int groups,
     int fold, int chunks, int width, int tiles) {
-  extern __shared__ float lds[];  // [2][parts * cols]
+  extern __shared__ float lds[];  // [2][parts * cols], [2][cols]
   const long long image = blockIdx.x / tiles;
   const int c0 = (int)(blockIdx.x % tiles) * width;
   const int cols = c - c0 < width ? c - c0 : width;
   const int cpg = c / groups;
-  const int parts = cols < kGroupBlock ? kGroupBlock / cols : 1;
+  const int threads = blockDim.x;
+  const int parts = cols < threads ? threads / cols : 1;
   // part[image][chunk][2][fold][c]
   const float* src = part + image * chunks * 2 * fold * c + c0;
   const float inv_fold = 1.f / (float)fold;
-  for (int i = threadIdx.x; i < parts * cols; i += kGroupBlock) {
+  for (int i = threadIdx.x; i < parts * cols; i += threads) {
     const int p = i / cols, col = i - p * cols;
     float a = 0.f, b = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int e = p; e < chunks * fold; e += parts) {
       const int ch = div_small(e, inv_fold);
       const float* at = src + ((long long)ch * 2 * fold + (e - ch * fold)) * c + col;
@@ -399,25 +417,35 @@ __global__ __launch_bounds__(kGroupBlock) void gn_bwd_group_kernel(
     lds[parts * cols + i] = b;
   }
   __syncthreads();
-  if (sums)
-    for (int col = threadIdx.x; col < cols; col += kGroupBlock) {
-      float a = 0.f, b = 0.f;
-      for (int p = 0; p < parts; ++p) {
-        a += lds[p * cols + col];
-        b += lds[(parts + p) * cols + col];
-      }
-      float* out = sums + image * 2 * c + c0 + col;
-      out[0] = a;
-      out[c] = b * rstd[image * groups + (c0 + col) / cpg];
-    }
-  const int lane = threadIdx.x % kWave;
-  for (int g = threadIdx.x / kWave; g < cols / cpg; g += kGroupBlock / kWave) {
+  // the columns' sums, 16 lanes each, in place where a column is one part
+  float* col_a = parts > 1 ? lds + 2 * parts * cols : lds;
+  float* col_b = col_a + cols;
+  for (int col = threadIdx.x / 16; col < cols; col += threads / 16) {
     float a = 0.f, b = 0.f;
-    for (int e = lane; e < parts * cpg; e += kWave) {
-      const int p = e / cpg, col = g * cpg + (e - p * cpg);
-      const float w = weight.at(c0 + col, 1.f);
-      a += w * lds[p * cols + col];
-      b += w * lds[(parts + p) * cols + col];
+    for (int p = threadIdx.x % 16; p < parts; p += 16) {
+      a += lds[p * cols + col];
+      b += lds[(parts + p) * cols + col];
+    }
+    a = lanes_sum<16>(a);
+    b = lanes_sum<16>(b);
+    if (threadIdx.x % 16 == 0) {
+      col_a[col] = a;
+      col_b[col] = b;
+      if (sums) {
+        float* out = sums + image * 2 * c + c0 + col;
+        out[0] = a;
+        out[c] = b * rstd[image * groups + (c0 + col) / cpg];
+      }
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x % kWave;
+  for (int g = threadIdx.x / kWave; g < cols / cpg; g += threads / kWave) {
+    float a = 0.f, b = 0.f;
+    for (int e = lane; e < cpg; e += kWave) {
+      const float w = weight.at(c0 + g * cpg + e, 1.f);
+      a += w * col_a[g * cpg + e];
+      b += w * col_b[g * cpg + e];
     }
     a = lanes_sum<kWave>(a);
     b = lanes_sum<kWave>(b);
@@ -548,14 +576,19 @@ hipError_t gn_fwd(const GnArgs& a, hipStream_t stream) {
   const GnPlan p = gn_plan(a);
   const int chunks = gn_short_chunks(a, p);
   if (gn_too_many(a.n * chunks * p.ctiles, kBlock) ||
-      gn_too_many((a.n * a.groups + 3) / 4, kBlock))
+      gn_too_many(a.n * a.groups, kWave))
     return hipErrorInvalidConfiguration;
   const dim3 fine((unsigned)(a.n * chunks * p.ctiles));
   const int coef = 3 * (int)sizeof(float) * p.cpb * p.vec;
   const Params weight = {a.weight, a.ptype}, bias = {a.bias, a.ptype};
   const dim3 grid((unsigned)(a.n * p.chunks * p.ctiles));
   const long long groups = a.n * a.groups;
-  const dim3 waves((unsigned)((groups + 3) / 4));
+  // Few groups of many chunks have 16 waves each: forward of 1x256x300x300 fp16
+  // takes 38 us so and 54 by one wave; where there are many, 42x800x42x43 bf16
+  // takes 82 us by one and 91 by 16.
+  const bool alone = groups <= 512 && p.fold * p.chunks > 128;
+  const int each = kBlock / kWave;  // groups a block, where they have one wave
+  const dim3 finals((unsigned)(alone ? groups : (groups + each - 1) / each));
   const int cpg = a.c / a.groups;
   const int cols = p.cpb * (cpg % p.vec == 0 ? 1 : p.vec);
   const int lds = columns_lds(kBlock, kBlock / p.cpb, cols);
@@ -564,7 +597,8 @@ hipError_t gn_fwd(const GnArgs& a, hipStream_t stream) {
             gn_stats_kernel<T, V><<<grid, kBlock, lds, stream>>>(
                 x, reinterpret_cast<Moments*>(a.ws), p.hw, p.c, cpg, p.cpb, p.ctiles,
                 p.chunks, p.span);
-            gn_finalize_kernel<<<waves, kBlock, 0, stream>>>(
+            const auto finalize = alone ? gn_finalize_kernel<16> : gn_finalize_kernel<1>;
+            finalize<<<finals, alone ? final_block<16>() : kBlock, 0, stream>>>(
                 reinterpret_cast<const Moments*>(a.ws), a.mean, a.rstd, groups, cpg, a.groups,
                 p.fold, p.cpb * p.vec, p.ctiles, p.chunks, p.span, a.eps);
             GN_ACT(a.act, gn_apply_kernel<T, V, A><<<fine, kBlock, coef, stream>>>(
@@ -589,12 +623,16 @@ hipError_t gn_bwd(const GnArgs& a, hipStream_t stream) {
     const int coef = (int)sizeof(float) * p.cpb * p.vec;  // LDS of one coefficient
     float2* k = reinterpret_cast<float2*>(a.ws + (a.n + gn_slices(a)) * 2 * a.c);
     float* part = reinterpret_cast<float*>(k + a.n * a.groups);
-    // whole groups of about 32 channels: many blocks, and many threads a
-    // channel, since the chunks are read one after another
+    // Whole groups of about 32 channels: many blocks, and many threads a
+    // channel, since the chunks are read one after another. More of both
+    // where there are few: backward of 1x288x150x150 fp16 34.0 us and 35.6
+    // without, 1x32x296x293 bf16 21.8 and 24.2.
     const int cpg = a.c / a.groups;
-    const int width = cpg >= 32 ? cpg : 32 / cpg * cpg;
+    const bool few = a.n * a.c < 32 * 128;
+    const int some = few ? 8 : 32, threads = few ? kGroupBlock : kGroupBlock / 2;
+    const int width = cpg >= some ? cpg : some / cpg * cpg;
     const int tiles = (a.c + width - 1) / width;
-    const int lds = 2 * (int)sizeof(float) * (width > kGroupBlock ? width : kGroupBlock);
+    const int lds = 2 * (int)sizeof(float) * (width > 2 * threads ? width : 2 * threads);
     if (gn_too_many(a.n * chunks * p.ctiles, kBlock) || gn_too_many(a.n * tiles, kGroupBlock))
       return hipErrorInvalidConfiguration;
     GN_TYPE(a.type, GN_VEC(p.vec, GN_ACT(a.act, {
@@ -603,7 +641,7 @@ hipError_t gn_bwd(const GnArgs& a, hipStream_t stream) {
               gn_bwd_sums_kernel<T, V, A><<<grid, kBlock, 3 * coef, stream>>>(
                   dy, x, weight, bias, a.drop, a.mean, a.rstd, part, p.hw, p.c, a.groups,
                   cpg, p.cpb, p.ctiles, p.chunks);
-              gn_bwd_group_kernel<<<dim3((unsigned)(a.n * tiles)), kGroupBlock, lds, stream>>>(
+              gn_bwd_group_kernel<<<dim3((unsigned)(a.n * tiles)), threads, lds, stream>>>(
                   part, weight, a.rstd, k, sums, a.hw, a.c, a.groups, p.fold, p.chunks, width,
                   tiles);
               if (a.dx)
