@@ -56,10 +56,6 @@ SlabPlan slab_plan(const GnArgs& a, int tensors) {
   if (a.hw >= (1 << 16) || a.c >= (1 << 14)) return best;
   const int widest = gn_vec(a);
   for (int vec = widest; vec >= 1; vec >>= 1) {
-    // Loads of less than 8 bytes are for small tensors, where time is a
-    // launch's: 32x336x38x38 bf16 (groups of 21 channels) by vectors of 2 takes
-    // 30 us forward and 67 backward, streaming 32 and 48.
-    if (vec < widest && vec * es < 8 && a.n * a.hw * a.c * es > (4 << 20)) break;
     const int unit = cpg / gcd_of(cpg, vec) * vec;
     // A row's part of a slab is 64 bytes or more, or 32 where it then fits. Of
     // many images of few rows a slab is 2 KB or more: a block has its own price.
@@ -81,6 +77,12 @@ SlabPlan slab_plan(const GnArgs& a, int tensors) {
       const long long bytes = a.hw * width * es;
       const int threads = blocks <= 64 ? 1024 : bytes <= 4096 ? 64 : bytes <= 16384 ? 256 : 512;
       if (!slab_try(a, tensors, vec, width, threads, &p)) continue;
+      // Loads of less than 8 bytes cost what wide ones do: of more than 16 a
+      // thread, streaming is faster. us by a slab and streaming, fp16, forward
+      // and backward: 1x1632x10x10 (5 rows a thread) 7.4 and 14.2, 8.8 and 19.4;
+      // 1x960x38x38 (21) 16.7 and 16.6, 25.4 and 22.0; 4x336x38x38 (30) 21.3
+      // and 16.2; backward of 1x192x75x75 (17) 31.5 and 21.4.
+      if (vec * es < 8 && a.hw > 16 * p.nrg) continue;
       // With less than a block for every other CU, narrower vectors make more
       // and smaller slabs.
       if (best.threads == 0 || (a.n * best.slices < 128 && p.slices > best.slices)) best = p;
