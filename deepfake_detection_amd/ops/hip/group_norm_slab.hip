@@ -57,8 +57,9 @@ SlabPlan slab_plan(const GnArgs& a, int tensors) {
   const int widest = gn_vec(a);
   for (int vec = widest; vec >= 1; vec >>= 1) {
     const int unit = cpg / gcd_of(cpg, vec) * vec;
-    // A row's part of a slab is 64 bytes or more, or 32 where it then fits. Of
-    // many images of few rows a slab is 2 KB or more: a block has its own price.
+    // A row's part of a slab is 64 bytes or more: backward of 64x256x38x38 bf16
+    // in parts of 32 bytes takes 90 us, streaming 61; less only for a few blocks.
+    // Of many images of few rows a slab is 2 KB or more: a block has its own price.
     int m = 1;
     while (m * unit < a.c &&
            (m * unit * es < 64 ||
@@ -68,7 +69,7 @@ SlabPlan slab_plan(const GnArgs& a, int tensors) {
       const int width = m * unit < a.c ? m * unit : a.c;
       const long long blocks = a.n * ((a.c + width - 1) / width);
       const bool few = blocks < 128;
-      if (width * es < 32 && width < a.c && !few) break;
+      if (width * es < 64 && width < a.c && !few) break;
       // 512 slabs of 13 KB: 12.7 us by 256 threads, 13.6 by 512; 256 of 29 KB:
       // 14.5 us by 512, 15.9 by 1024; 28 of 80 KB: 13.9 us by 1024; 8192 of
       // 3 KB (1024x256x7x7 bf16): 20.8 us by 64, 24.6 by 128, 36.8 by 256;
@@ -77,12 +78,18 @@ SlabPlan slab_plan(const GnArgs& a, int tensors) {
       const long long bytes = a.hw * width * es;
       const int threads = blocks <= 64 ? 1024 : bytes <= 4096 ? 64 : bytes <= 16384 ? 256 : 512;
       if (!slab_try(a, tensors, vec, width, threads, &p)) continue;
-      // Loads of less than 8 bytes cost what wide ones do: of more than 16 a
-      // thread, streaming is faster. us by a slab and streaming, fp16, forward
-      // and backward: 1x1632x10x10 (5 rows a thread) 7.4 and 14.2, 8.8 and 19.4;
-      // 1x960x38x38 (21) 16.7 and 16.6, 25.4 and 22.0; 4x336x38x38 (30) 21.3
-      // and 16.2; backward of 1x192x75x75 (17) 31.5 and 21.4.
-      if (vec * es < 8 && a.hw > 16 * p.nrg) continue;
+      // Narrow loads cost what wide ones do: of more than 16 a thread, streaming
+      // is faster. us by a slab and streaming, forward and backward: fp16
+      // 1x1632x10x10 (5 rows a thread) 7.4 and 14.2, 8.8 and 19.4; 1x960x38x38
+      // (21) 16.7 and 16.6, 25.4 and 22.0; 4x336x38x38 (30) 21.3 and 16.2;
+      // backward of 1x192x75x75 (17) 31.5 and 21.4; fp32 46x96x41x43 (31) 39.2
+      // and 27.4.
+      if (vec * es < 16 && a.hw > 16 * p.nrg) continue;
+      // One block alone on a CU does not hide its chain. us by a slab and
+      // streaming, bf16: forward of 64x1020x25x25 in 960 blocks 80 and 58,
+      // backward of 128x256x24x24 in 1024 60 and 53, of 32x512x28x28 in 512 36
+      // and 46, of 128x1632x10x10 in 1024 63 and 70.
+      if (2 * p.lds > kLds && blocks > 512) continue;
       // With less than a block for every other CU, narrower vectors make more
       // and smaller slabs.
       if (best.threads == 0 || (a.n * best.slices < 128 && p.slices > best.slices)) best = p;
