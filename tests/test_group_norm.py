@@ -459,6 +459,24 @@ def test_gradients_of_gradients_are_refused():
 
 
 @pytest.mark.gpu
+def test_without_a_gradient():
+    """The call that keeps nothing gives the bits of the one that does; forward
+    derivatives are refused by both."""
+    for shape in (SHAPES[4], SHAPES[9]):
+        x, gn, dy, residual, drop = make(shape, torch.bfloat16, "cuda", "silu", tail=True)
+        want = step(x, gn, "silu", dy, residual, drop)["y"]
+        with torch.no_grad():
+            assert torch.equal(O.group_norm_act(x, gn, "silu", residual, drop), want)
+        gn.requires_grad_(False)
+        got = O.group_norm_act(x, gn, "silu", residual, drop)
+        assert torch.equal(got, want) and not got.requires_grad
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x, dy)
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                O.group_norm_act(dual, gn, "silu")
+
+
+@pytest.mark.gpu
 def test_captured_and_replayed():
     """Two graphs of the op, replayed in turn with new inputs between eager
     calls, give the eager results."""
