@@ -616,3 +616,129 @@ def test_train_runner_with_a_teacher(tmp_path):
         "--input-size-v2", "3,32,32", "-j", "0", "--no-amp", "--sched", "step",
         "--output", str(tmp_path), "--model-version", "t"])
     assert (tmp_path / "t-resnet18" / "summary.csv").exists()
+
+
+# ---------------------------------------------------------------------------
+# finite masks and large logits
+# ---------------------------------------------------------------------------
+
+def masked_answers(device, dtype, mask, t, classes, k=6):
+    """Students whose classes are switched off by a finite value in the ways
+    that programs do it, and a teacher's answers."""
+    z = logits_of(7, classes, dtype, device, seed=1)
+    answer = answers(7, classes, k, dtype, device, t)
+    named = answer[1]
+    keep = z.gather(1, named)
+    few = torch.tensor([1, classes // 3, classes - 2], device=device)
+    few_keep = z[3, few].clone()
+    z[0, :classes // 2] = mask   # the first classes of a head
+    z[1, classes // 2:] = mask   # its padding
+    z[2] = mask                  # all that the teacher does not name
+    z[3] = mask                  # and all but three of them
+    z[3, few] = few_keep
+    z[4, ::2] = mask
+    z[5, classes // 2] = mask
+    z[6] = mask                  # one class alone is left
+    z.scatter_(1, named, keep)
+    z[6, named[6, 1:]] = mask
+    return z, answer
+
+
+def check_far(logits, values, indices, rest, t, far_answer=True):
+    """check_distill for rows far from 0, of which 64 bits keep the differences
+    alone: the oracle takes them from the row's largest.
+
+    With far_answer u = v / T is so large that its own roundings count: 1 / T,
+    the product and the difference from the largest are each off by 2^-24 of
+    |u| or less, of u_j and of u_top, so q has a factor within exp(8 U |u|), and
+    so have the terms of the loss and of the gradient."""
+    up = torch.rand(logits.shape[0], generator=torch.Generator().manual_seed(0)) + 0.5
+    near = logits.detach().double()
+    near = near - near.amax(1, keepdim=True)
+    want_loss, want_grad, loss_size, grad_size = distill_oracle(
+        near, values, indices, rest, t, up)
+    leaf = logits.detach().requires_grad_()
+    loss = O.distill_topk(leaf, values, indices, rest, t)
+    (grad,) = torch.autograd.grad(loss, leaf, up.to(leaf.device))
+    n = sum_length(logits.shape[1])
+    size = torch.maximum((values.double() / t).abs().amax(1), rest.double().abs()).cpu()
+    factor = torch.expm1(8 * U * size) * far_answer
+    off = (loss.detach().cpu().double() - want_loss).abs()
+    assert (off <= U * (32 * loss_size + 2 * n) + factor * loss_size).all()
+    off = (grad.cpu().double() - want_grad).abs()
+    allowed = torch.finfo(grad.dtype).eps / 2 * want_grad.abs() + 2.0 ** -125 * (up.double() / t)[:, None]
+    allowed = allowed + (2 * U * (32 + n) + factor[:, None]) * grad_size
+    assert (off <= allowed).all(), (off / allowed).max()
+
+
+def finite_masks(device, dtype, mask, t, classes, check=check_distill):
+    z, answer = masked_answers(device, dtype, mask, t, classes)
+    # 3e38 / 0.25 is beyond the 3.4e38 of the fp32 that the loss and its
+    # logarithms have: rows that teach a masked class have an infinite loss
+    rows = torch.arange(7, device=device)
+    if abs(float(z[2].min())) / t > torch.finfo(torch.float32).max:
+        rows = rows[[0, 1, 3, 4, 5]]
+    check(z[rows], *(a[rows] for a in answer), t)
+    leaf = z.requires_grad_()
+    up = torch.rand(7, generator=torch.Generator().manual_seed(0)).to(device) + 0.5
+    up = up * 64 if dtype == torch.float16 else up
+    loss = O.distill_topk(leaf, *answer, temperature=t)
+    (grad,) = torch.autograd.grad(loss, leaf, up)
+    assert torch.isfinite(loss[rows]).all() and torch.isfinite(grad).all()
+    assert (loss[[i for i in (2, 6) if i not in rows.tolist()]] == INF).all()
+    # Where all of the rest are equal and far below, their gradient is
+    # -(g / T) q_r / (how many). q_r = exp(u_r - u_top) / sum has the roundings
+    # of u = v (1 / T) in its exponent, four of |u| at most, and some of its own.
+    values, indices, rest = (a[2].double().cpu() for a in answer)
+    up = up[2].double().cpu()
+    q_rest = torch.softmax(torch.cat([values / t, rest[None]]), 0)[-1]
+    others = torch.ones(classes, dtype=torch.bool)
+    others[indices.long()] = False
+    want = -q_rest * up / t / others.sum()
+    off = (grad[2].double().cpu()[others] - want).abs()
+    least = torch.finfo(dtype).tiny * torch.finfo(dtype).eps + 2.0 ** -126 * up / t
+    size = (values / t).abs().max() + rest.abs()
+    if mask < 0:
+        assert (off <= (torch.finfo(dtype).eps / 2 + U * (32 + 4 * size)) * want.abs() + least).all()
+
+
+MASKS = [-1e6, -1e9, -1e10, -1e12, -1e20, -1e25, -1e30, -3e38, 1e10, 1e20]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("classes", [203, 1203, 20011])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("mask", MASKS, ids=str)
+def test_finite_masks(mask, dtype, classes):
+    for t in (0.25, 0.5, 1.0, 2.0, 4.0):
+        finite_masks("cuda", TYPES[dtype], mask, t, classes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mask", [-6e4, -65504.0, -3e4])
+def test_finite_masks_fp16(mask):
+    for t in (0.01, 0.25, 1.0):  # the gradient, 96 / T at most, fits the type
+        finite_masks("cuda", torch.float16, mask, t, 1203)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("t", [1e-6, 1e-4, 1e-2])
+def test_small_temperatures(t, dtype):
+    """Ordinary masks over a small temperature are as far away as large ones."""
+    for mask in (-1e4, -6e4, 3e4):
+        finite_masks("cuda", TYPES[dtype], mask, t, 1203, check=check_far)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("offset", [s * 10.0 ** e for s in (1, -1) for e in (4, 6, 8, 9, 10, 12, 20, 30, 38)],
+                         ids=str)
+def test_logits_of_a_common_offset(offset, dtype):
+    """A row far from 0 is the same row: what its type keeps of it."""
+    for t in (0.25, 1.0, 4.0):
+        z = logits_of(4, 1203, torch.float32, "cuda", seed=1)
+        answer = answers(4, 1203, 6, TYPES[dtype], "cuda", t)
+        z = (z + offset).to(TYPES[dtype])
+        check_far(z, *answer, t, far_answer=False)
+        check_topk(z, 6, t)
