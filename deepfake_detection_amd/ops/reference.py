@@ -79,9 +79,19 @@ def distill_topk_forward(logits, values, indices, rest=None, temperature=1.0):
     named = named.scatter_add_(1, at, slot.to(wide)) > 0
     # where the teacher leaves the rest nothing its sum has no part in the loss
     counts = (q[:, -1:] > 0) & named & teaches[:, None]
-    log_rest = torch.logsumexp(z.masked_fill(counts, -inf), dim=1, keepdim=True)
-    log_p = torch.cat([z.gather(1, at), log_rest], dim=1) - torch.logsumexp(
-        z, dim=1, keepdim=True)
+    others = z.masked_fill(counts, -inf)
+
+    # both sums about their largest: the gradient of logsumexp takes exp(z - its
+    # result), which far from 0 is rounded to steps of more than one
+    def largest(v):
+        top = v.detach().amax(dim=1, keepdim=True)
+        return torch.where(top.isfinite(), top, 0.0)
+
+    top, top_rest = largest(z), largest(others)
+    near = z - top
+    log_rest = torch.logsumexp(others - top_rest, dim=1, keepdim=True) + (top_rest - top)
+    log_p = torch.cat([near.gather(1, at), log_rest], dim=1) - torch.logsumexp(
+        near, dim=1, keepdim=True)
     # q log q - q log p, with 0 for q = 0
     loss = torch.where(q == 0, 0.0, torch.xlogy(q, q) - q * log_p).sum(dim=1)
     loss = torch.where(teaches | bad, loss, 0.0)

@@ -705,6 +705,12 @@ def finite_masks(device, dtype, mask, t, classes, check=check_distill):
 MASKS = [-1e6, -1e9, -1e10, -1e12, -1e20, -1e25, -1e30, -3e38, 1e10, 1e20]
 
 
+@pytest.mark.parametrize("mask", MASKS[::2], ids=str)
+def test_finite_masks_cpu(mask):
+    for t in (0.25, 1.0, 4.0):
+        finite_masks("cpu", torch.float32, mask, t, 1203)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("classes", [203, 1203, 20011])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
