@@ -44,9 +44,17 @@ def _needs_rebuild(obj, src, headers):
 
 
 def _headers_of(src):
-    with open(src) as f:
-        names = re.findall(r'#include "(\w+\.h)"', f.read())
-    return [os.path.join(SRC_DIR, name) for name in names]
+    """The headers of SRC_DIR that src includes, and those that they include."""
+    found = []
+    left = [src]
+    while left:
+        with open(left.pop()) as f:
+            names = re.findall(r'^\s*#\s*include\s+"([^"]+)"', f.read(), re.MULTILINE)
+        for path in (os.path.join(SRC_DIR, name) for name in names):
+            if path not in found and os.path.exists(path):
+                found.append(path)
+                left.append(path)
+    return found
 
 
 def build(verbose=True, force=False):
