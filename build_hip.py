@@ -87,6 +87,8 @@ def build(verbose=True, force=False):
             force = force or f.read() != flags
     else:
         force = True
+    if force and os.path.exists(stamp):
+        os.remove(stamp)  # an interrupted build leaves objects of both flags
     objs = []
     cmds = []
     for src in SOURCES:
@@ -104,11 +106,13 @@ def build(verbose=True, force=False):
     # the sources are independent and some take minutes
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
         list(pool.map(compile_one, cmds))
-    compiled = len(cmds)
     with open(stamp, "w") as f:
         f.write(flags)
 
-    if compiled or not os.path.exists(OUT_SO) or force:
+    # an object may be newer without having been compiled here: the last build's
+    # link may have failed
+    if (not os.path.exists(OUT_SO)
+            or any(os.path.getmtime(o) > os.path.getmtime(OUT_SO) for o in objs)):
         link = [hipcc, "-shared", "-fPIC", "-o", OUT_SO] + objs + [
             f"-L{lib_dir}", "-ltorch", "-ltorch_hip", "-lc10", "-lc10_hip",
             "-ltorch_python", f"-Wl,-rpath,{lib_dir}",

@@ -1,20 +1,23 @@
-"""The extension's build: what a changed file makes it compile again. A script takes the compiler's place."""
+"""The extension's build: what a changed file, changed flags or an interrupted
+build make it compile again. A script takes the compiler's place."""
 
 import os
 import shutil
 import stat
+import subprocess
 
 import pytest
 
 import build_hip
 
 COMPILER = """#!/bin/sh
-# writes the file after -o
+# writes the file after -o; fails for a name that holds $FAIL
 out=
 while [ $# -gt 0 ]; do
   if [ "$1" = -o ]; then out=$2; fi
   shift
 done
+case "$out" in *"${FAIL:-no such name}"*) exit 1;; esac
 echo "$(basename "$out")" >> "$LOG"
 echo built > "$out"
 """
@@ -44,6 +47,9 @@ def tree(tmp_path, monkeypatch):
 
     build.src = src
     assert len(build()) == len(build_hip.SOURCES) + 1
+    for f in (tmp_path / "build").glob("*.o"):
+        os.utime(f, (f.stat().st_mtime - 60,) * 2)
+    os.utime(build_hip.OUT_SO, (os.stat(build_hip.OUT_SO).st_mtime - 30,) * 2)
     return build
 
 
@@ -71,3 +77,24 @@ def test_header_of_a_header(tree):
 def test_header_of_all(tree):
     touch(tree.src / "common.h")
     assert {"group_norm.o", "group_norm_slab.o", "distill.o", "bn_act.o", "ops.so"} <= tree()
+
+
+def test_an_interrupted_build_with_other_flags(tree, monkeypatch):
+    """Some objects have the new flags when it ends: going back compiles them
+    again, too."""
+    monkeypatch.setattr(build_hip, "ARCH", "other")
+    monkeypatch.setenv("FAIL", "small_batch.o")
+    with pytest.raises(subprocess.CalledProcessError):
+        tree()
+    monkeypatch.setattr(build_hip, "ARCH", "gfx950")
+    monkeypatch.delenv("FAIL")
+    assert len(tree()) == len(build_hip.SOURCES) + 1
+
+
+def test_an_interrupted_link(tree, monkeypatch):
+    touch(tree.src / "distill.hip")
+    monkeypatch.setenv("FAIL", "ops.so")
+    with pytest.raises(subprocess.CalledProcessError):
+        tree()
+    monkeypatch.delenv("FAIL")
+    assert tree() == {"ops.so"}
