@@ -110,15 +110,35 @@ class GroupNorm2d(nn.GroupNorm):
         super().__init__(math.gcd(num_features, num_groups), num_features, eps, affine)
 
     def forward(self, x):
+        self.check_spread(x)
         return O.group_norm_act(x, self, "none")
+
+    def check_spread(self, x):
+        """Refuse to train where each group is one value: the output would be
+        the bias, whatever the input, and no gradient would pass."""
+        if (self.training and self.num_groups == self.num_channels
+                and x.dim() == 4 and x.shape[2] == 1 and x.shape[3] == 1):
+            raise ValueError(f"GroupNorm2d: one value a group: {self.num_groups} groups of "
+                             f"{self.num_channels} channels at 1x1")
+
+
+def _pooled_norm(norm_layer, num_features):
+    """The norm of globally pooled features, which have one value a channel: a
+    BatchNorm2d, or a group norm of one group."""
+    if getattr(norm_layer, "func", norm_layer) is GroupNorm2d:
+        return norm_layer(num_features, num_groups=1)
+    norm = nn.BatchNorm2d(num_features)
+    norm.pooled = True  # for convert_groupnorm_model
+    return norm
 
 
 def convert_groupnorm_model(module, num_groups=32):
     """Replace every BatchNorm2d by a GroupNorm2d that keeps its eps and its
-    weight and bias; running statistics are dropped. Returns the model."""
+    weight and bias; running statistics are dropped. Those of pooled features
+    have one group. Returns the model."""
     if type(module) is nn.BatchNorm2d:
         mod = GroupNorm2d(module.num_features, module.eps, affine=module.affine,
-                          num_groups=num_groups)
+                          num_groups=1 if getattr(module, "pooled", False) else num_groups)
         mod.train(module.training)
         if module.affine:
             mod.weight, mod.bias = module.weight, module.bias
@@ -274,7 +294,7 @@ class SelectiveKernelConv(nn.Module):
 
         attn_channels = max(int(out_channels / attn_reduction), min_attn_channels)
         self.fc_reduce = nn.Conv2d(out_channels, attn_channels, kernel_size=1, bias=False)
-        self.bn = nn.BatchNorm2d(attn_channels)
+        self.bn = _pooled_norm(norm_layer, attn_channels)
         self.act = act_layer(inplace=True)
         self.fc_select = nn.Conv2d(attn_channels, out_channels * self.num_paths,
                                    kernel_size=1, bias=False)

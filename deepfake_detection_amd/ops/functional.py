@@ -52,6 +52,7 @@ def bn_act(x, bn, act: str = "silu", residual=None, drop_path_mask=None):
     the residual add. A GroupNorm2d in bn's place runs as group_norm_act."""
     if not fusable_bn(bn):
         if fusable_gn(bn) and act in _FUSED_ACTS:
+            bn.check_spread(x)
             return group_norm_act(x, bn, act, residual, drop_path_mask)
         # Subclass with its own semantics (SplitBatchNorm2d, SyncBatchNorm...):
         # module dispatch, then the named activation.

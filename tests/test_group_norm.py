@@ -256,6 +256,51 @@ def test_model_built_with_group_norm():
     assert model(torch.randn(1, 3, 64, 64)).shape == (1, 4)
 
 
+def has_a_live_gradient(model, x):
+    model.train()
+    model(x).square().sum().backward()
+    dead = [k for k, p in model.named_parameters() if not p.grad.abs().max() > 0]
+    assert not dead, dead
+
+
+@pytest.mark.parametrize("name", ["skresnet18", "skresnet50"])
+def test_norms_of_pooled_features_keep_their_spread(name):
+    """Pooled features have one value a channel: as many groups as channels
+    would leave of them their bias alone."""
+    import deepfake_detection_amd as dfd
+
+    torch.manual_seed(0)
+    x = torch.randn(2, 3, 64, 64)
+    for groups in (32, 8):
+        model = convert_groupnorm_model(dfd.create_model(name, num_classes=4), groups)
+        assert not any(isinstance(m, nn.BatchNorm2d) for m in model.modules())
+        has_a_live_gradient(model, x)
+    model = dfd.create_model(name, num_classes=4, norm_layer=GroupNorm2d)
+    assert not any(isinstance(m, nn.BatchNorm2d) for m in model.modules())
+    has_a_live_gradient(model, x)
+
+
+@pytest.mark.parametrize("name", ["efficientnet_b0", "resnet18", "efficientnet_lite0"])
+def test_converted_model_has_a_live_gradient(name):
+    import deepfake_detection_amd as dfd
+
+    torch.manual_seed(0)
+    model = convert_groupnorm_model(dfd.create_model(name, num_classes=4))
+    has_a_live_gradient(model, torch.randn(2, 3, 64, 64))
+
+
+def test_one_value_a_group_is_refused_in_training():
+    norm = GroupNorm2d(32)
+    x = torch.randn(2, 32, 1, 1)
+    with pytest.raises(ValueError, match="one value"):
+        norm(x)
+    with pytest.raises(ValueError, match="one value"):
+        O.bn_act(x, norm, "silu")
+    assert torch.equal(norm.eval()(x), norm.bias.view(1, 32, 1, 1).expand(2, 32, 1, 1))
+    assert GroupNorm2d(32)(torch.randn(2, 32, 1, 2)).abs().max() > 0
+    assert GroupNorm2d(48)(torch.randn(2, 48, 1, 1)).abs().max() > 0
+
+
 def test_relu6_keeps_its_bound():
     from deepfake_detection_amd.models.blocks import ConvBnAct
 
