@@ -16,27 +16,44 @@ import torch
 _logger = logging.getLogger(__name__)
 
 
-def load_state_dict(checkpoint_path, use_ema=False):
+def _read_checkpoint(checkpoint_path):
     if checkpoint_path and os.path.isfile(checkpoint_path):
-        checkpoint = torch.load(checkpoint_path, map_location="cpu", weights_only=False)
-        state_dict_key = ""
-        if isinstance(checkpoint, dict):
-            if use_ema and "state_dict_ema" in checkpoint:
-                state_dict_key = "state_dict_ema"
-            elif "state_dict" in checkpoint:
-                state_dict_key = "state_dict"
-        if state_dict_key:
-            new_state_dict = OrderedDict()
-            for k, v in checkpoint[state_dict_key].items():
-                name = k[7:] if k.startswith("module.") else k
-                new_state_dict[name] = v
-            state_dict = new_state_dict
-        else:
-            state_dict = checkpoint
-        _logger.info("Loaded %s from checkpoint '%s'", state_dict_key or "weights", checkpoint_path)
-        return state_dict
+        return torch.load(checkpoint_path, map_location="cpu", weights_only=False)
     _logger.error("No checkpoint found at '%s'", checkpoint_path)
     raise FileNotFoundError(checkpoint_path)
+
+
+def _weights_of(checkpoint, checkpoint_path, use_ema=False):
+    state_dict_key = ""
+    if isinstance(checkpoint, dict):
+        if use_ema and "state_dict_ema" in checkpoint:
+            state_dict_key = "state_dict_ema"
+        elif "state_dict" in checkpoint:
+            state_dict_key = "state_dict"
+    if state_dict_key:
+        new_state_dict = OrderedDict()
+        for k, v in checkpoint[state_dict_key].items():
+            name = k[7:] if k.startswith("module.") else k
+            new_state_dict[name] = v
+        state_dict = new_state_dict
+    else:
+        state_dict = checkpoint
+    _logger.info("Loaded %s from checkpoint '%s'", state_dict_key or "weights", checkpoint_path)
+    return state_dict
+
+
+def load_state_dict(checkpoint_path, use_ema=False):
+    return _weights_of(_read_checkpoint(checkpoint_path), checkpoint_path, use_ema)
+
+
+def load_with_args(checkpoint_path):
+    """(weights, args) of a checkpoint: args are those of the training run that
+    wrote it, as a dict, or {} where it holds none."""
+    checkpoint = _read_checkpoint(checkpoint_path)
+    args = checkpoint.get("args") if isinstance(checkpoint, dict) else None
+    if args is not None and not isinstance(args, dict):
+        args = vars(args)
+    return _weights_of(checkpoint, checkpoint_path), dict(args or {})
 
 
 def load_checkpoint(model, checkpoint_path, use_ema=False, strict=True, ignore_keys=None):

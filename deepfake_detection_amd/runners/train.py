@@ -46,6 +46,7 @@ from ..parallel.distributed import convert_sync_batchnorm
 from ..scheduler import create_scheduler
 from ..utils import CheckpointSaver, ModelEma, setup_default_logging, update_summary
 from ..models import resume_checkpoint
+from ..models.helpers import load_with_args
 
 _logger = logging.getLogger("train")
 
@@ -132,9 +133,14 @@ def _build_parser():
     # Distillation
     parser.add_argument("--teacher", default="", type=str, metavar="MODEL",
                         help="model whose answers the trained one learns from too")
-    parser.add_argument("--teacher-checkpoint", default="", type=str, metavar="PATH")
+    parser.add_argument("--teacher-checkpoint", default="", type=str, metavar="PATH",
+                        help="its weights, all of them; on synthetic data it may do without")
     parser.add_argument("--teacher-group-norm", type=int, default=0, metavar="G",
-                        help="the teacher was trained with --group-norm G")
+                        help="the teacher was trained with --group-norm G; this and the next "
+                             "three default to what its checkpoint says of its training")
+    parser.add_argument("--teacher-bn-tf", action="store_true", default=False)
+    parser.add_argument("--teacher-bn-eps", type=float, default=None)
+    parser.add_argument("--teacher-gp", default=None, type=str, metavar="POOL")
     parser.add_argument("--distill-k", type=int, default=20, metavar="K",
                         help="the teacher's K largest logits are learned")
     parser.add_argument("--distill-temperature", type=float, default=2.0, metavar="T")
@@ -351,13 +357,7 @@ def main(rank, args, args_text, world_size=None, start_rank=0):
     teacher = None
     if args.teacher:
         assert not args.jsd, "--jsd's loss already compares the model with itself"
-        teacher = create_model(
-            args.teacher, num_classes=args.num_classes, in_chans=in_chans,
-            checkpoint_path=args.teacher_checkpoint)
-        if args.teacher_group_norm:
-            from ..models.layers_extra import convert_groupnorm_model
-
-            teacher = convert_groupnorm_model(teacher, args.teacher_group_norm)
+        teacher = _build_teacher(args, in_chans)
         teacher = teacher.to(device).eval().requires_grad_(False)
         if use_cuda:
             teacher = teacher.to(memory_format=torch.channels_last)
@@ -433,6 +433,37 @@ def main(rank, args, args_text, world_size=None, start_rank=0):
         pass
     if best_metric is not None:
         _logger.info("*** Best metric: {0} (epoch {1})".format(best_metric, best_epoch))
+
+
+def _build_teacher(args, in_chans):
+    """The model of --teacher, as it was trained, with all of its weights."""
+    if not args.teacher_checkpoint:
+        if not (args.synthetic_data or args.data is None):
+            raise ValueError("--teacher needs --teacher-checkpoint: nothing is to be learned "
+                             "from random weights")
+        _logger.warning("the teacher has random weights")
+        weights, trained = None, {}
+    else:
+        weights, trained = load_with_args(args.teacher_checkpoint)
+    if trained.get("model", args.teacher) != args.teacher:
+        raise ValueError(f"--teacher {args.teacher}: {args.teacher_checkpoint} is of a "
+                         f"{trained['model']}")
+    bn_eps = args.teacher_bn_eps
+    teacher = create_model(
+        args.teacher, num_classes=args.num_classes, in_chans=in_chans,
+        global_pool=args.teacher_gp or trained.get("gp") or "avg",
+        bn_tf=args.teacher_bn_tf or trained.get("bn_tf", False),
+        bn_eps=trained.get("bn_eps") if bn_eps is None else bn_eps)
+    group_norm = args.teacher_group_norm or trained.get("group_norm", 0)
+    if group_norm:
+        from ..models.layers_extra import convert_groupnorm_model
+
+        teacher = convert_groupnorm_model(teacher, group_norm)
+    if weights is not None:
+        # a split BatchNorm's other parts are of training alone
+        weights = {k: v for k, v in weights.items() if ".aux_bn." not in k}
+        teacher.load_state_dict(weights, strict=True)
+    return teacher
 
 
 def _synthetic_loader(dataset, args, data_config, is_training):

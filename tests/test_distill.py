@@ -748,3 +748,109 @@ def test_logits_of_a_common_offset(offset, dtype):
         z = (z + offset).to(TYPES[dtype])
         check_far(z, *answer, t, far_answer=False)
         check_topk(z, 6, t)
+
+
+# ---------------------------------------------------------------------------
+# the teacher of a training run
+# ---------------------------------------------------------------------------
+
+def teacher_of(*flags):
+    from deepfake_detection_amd.runners.train import _build_teacher, _parse_args
+
+    args, _ = _parse_args(["--data", "frames", *map(str, flags)])
+    return _build_teacher(args, 3).eval()
+
+
+def trained_model(name, group_norm=0, **kw):
+    """A model whose weights and statistics are not those it was made with."""
+    import deepfake_detection_amd as dfd
+    from deepfake_detection_amd.models.layers_extra import convert_groupnorm_model
+
+    torch.manual_seed(3)
+    model = dfd.create_model(name, num_classes=2, **kw)
+    if group_norm:
+        model = convert_groupnorm_model(model, group_norm)
+    with torch.no_grad():
+        for k, v in model.state_dict().items():
+            if k.endswith("running_var"):
+                v.uniform_(0.001, 0.5)
+            elif v.is_floating_point() and v.dim() == 1:
+                v.add_(torch.rand_like(v) * 0.1)
+    return model.eval()
+
+
+@pytest.mark.parametrize("flags,kw", [
+    ([], {}),
+    (["--bn-tf"], {"bn_tf": True}),
+    (["--bn-eps", "0.01"], {"bn_eps": 0.01}),
+    (["--gp", "max"], {"global_pool": "max"}),
+    (["--group-norm", "8"], {"group_norm": 8}),
+], ids=str)
+def test_teacher_answers_as_it_was_trained(tmp_path, flags, kw):
+    """By what its checkpoint says of its training, or by the teacher's flags."""
+    from deepfake_detection_amd.runners.train import _parse_args
+
+    name = "efficientnet_b0"
+    model = trained_model(name, **kw)
+    x = torch.randn(2, 3, 64, 64)
+    want = model(x)
+    path = tmp_path / "teacher.pth.tar"
+    state = {"module." + k: v for k, v in model.state_dict().items()}
+    torch.save({"state_dict": state, "args": _parse_args(["--model", name, *flags])[0]}, path)
+    got = teacher_of("--teacher", name, "--teacher-checkpoint", path)(x)
+    assert torch.equal(got, want)
+    torch.save(model.state_dict(), path)  # weights alone
+    got = teacher_of("--teacher", name, "--teacher-checkpoint", path,
+                     *[f.replace("--", "--teacher-") for f in flags])(x)
+    assert torch.equal(got, want)
+
+
+def test_teacher_of_a_split_norm(tmp_path):
+    from deepfake_detection_amd.models.layers_extra import convert_splitbn_model
+
+    model = trained_model("resnet18")
+    x = torch.randn(2, 3, 64, 64)
+    want = model(x)
+    path = tmp_path / "teacher.pth.tar"
+    torch.save(convert_splitbn_model(model, 2).state_dict(), path)
+    assert torch.equal(teacher_of("--teacher", "resnet18", "--teacher-checkpoint", path)(x), want)
+
+
+def test_teachers_that_are_refused(tmp_path):
+    from deepfake_detection_amd.runners.train import _parse_args
+
+    path = tmp_path / "teacher.pth.tar"
+    with pytest.raises(ValueError, match="--teacher-checkpoint"):
+        teacher_of("--teacher", "resnet18")
+    with pytest.raises(FileNotFoundError):
+        teacher_of("--teacher", "resnet18", "--teacher-checkpoint", path)
+    model = trained_model("resnet18")
+
+    def refused(state, match, *flags):
+        torch.save(state, path)
+        with pytest.raises((RuntimeError, ValueError), match=match):
+            teacher_of("--teacher", "resnet18", "--teacher-checkpoint", path, *flags)
+
+    weights = model.state_dict()
+    refused(trained_model("resnet34").state_dict(), "Unexpected key")
+    refused(trained_model("efficientnet_b0").state_dict(), "Missing key")
+    refused({k: v for k, v in weights.items() if k != "layer2.0.conv1.weight"}, "Missing key")
+    refused({**weights, "fc.weight": torch.zeros(5, 512)}, "size mismatch")
+    refused(trained_model("resnet18", group_norm=8).state_dict(), "Missing key")
+    refused(weights, "Unexpected key", "--teacher-group-norm", 8)
+    refused({"state_dict": weights, "args": _parse_args(["--model", "tf_efficientnet_b0"])[0]},
+            "is of a tf_efficientnet_b0")
+
+
+def test_train_runner_with_a_teacher_checkpoint(tmp_path):
+    from deepfake_detection_amd.runners.train import launch_main
+
+    path = tmp_path / "teacher.pth.tar"
+    torch.save(trained_model("resnet18", group_norm=16).state_dict(), path)
+    launch_main([
+        "--model", "resnet18", "--teacher", "resnet18", "--teacher-checkpoint", str(path),
+        "--teacher-group-norm", "16", "--synthetic-data", "--synthetic-len", "8", "-b", "4",
+        "--epochs", "1", "--warmup-epochs", "0", "--cooldown-epochs", "0",
+        "--input-size-v2", "3,32,32", "-j", "0", "--no-amp", "--sched", "step",
+        "--output", str(tmp_path), "--model-version", "t"])
+    assert (tmp_path / "t-resnet18" / "summary.csv").exists()
