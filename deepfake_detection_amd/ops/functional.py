@@ -194,7 +194,8 @@ def topk_logits(logits, k: int, temperature: float = 1.0):
 
     NaN counts as the largest value. logits: [..., classes], any row spacing;
     1 <= k <= 256 and no more than classes. No gradient: what a teacher says is
-    given. GPU: one pass over the logits (ops/hip/distill.hip).
+    given. GPU: one pass over the logits (ops/hip/distill.hip), fewer than
+    2^31 - 4096 classes.
     """
     _check_logits("topk_logits", logits, k, temperature)
     if k > logits.shape[-1]:

@@ -153,7 +153,8 @@ at::Tensor sized(const at::Tensor& t, at::IntArrayRef sizes) {
 at::Tensor as_rows(const at::Tensor& x, const char* who) {
   TORCH_CHECK(x.is_cuda() && x.dim() >= 1, who, ": CUDA logits expected");
   const int64_t classes = x.size(-1);
-  TORCH_CHECK(classes >= 1 && classes <= INT_MAX - 64, who, ": ", classes, " classes");
+  // a block's threads step past the last class by less than 4096, in 32 bits
+  TORCH_CHECK(classes >= 1 && classes <= INT_MAX - 4096, who, ": ", classes, " classes");
   auto rows = x.dim() == 2 ? x : x.reshape({-1, classes});
   TORCH_CHECK(rows.size(0) <= INT_MAX, who, ": too many rows");
   return rows.stride(1) == 1 || classes == 1 ? rows : rows.contiguous();

@@ -157,6 +157,16 @@ def test_topk_special_rows(classes, k, dtype):
 
 
 @pytest.mark.gpu
+def test_topk_of_rows_at_the_end_of_32_bits_is_refused():
+    """Threads step through a row by up to 512 classes; the next step must not
+    pass 2^31. (One element, expanded: nothing of that size is made.)"""
+    z = torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16)
+    for classes in (2 ** 31 - 65, 2 ** 31 - 512, 2 ** 31 - 4096):
+        with pytest.raises(RuntimeError, match="classes"):
+            O.topk_logits(z.expand(1, classes), 3)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_topk_where_one_thread_owns_the_largest(dtype):
     """The k largest lie where one thread's vectors would: its fellows' largest
