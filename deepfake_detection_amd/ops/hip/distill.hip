@@ -674,7 +674,8 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
   __syncthreads();
   for (int j = tid; j < k; j += THREADS) {
     const long long at = indices[r * k + j];
-    if (at < 0) continue;
+    // (the forward pass has looked at them, but they may have changed since)
+    if (at < 0 || at >= classes) continue;
     float q = 0.f;
     if (s.state == kTwice) {
       for (int i = 0; i < k; ++i)

@@ -414,6 +414,25 @@ def test_distill_special_rows(classes, dtype):
 
 
 @pytest.mark.gpu
+def test_distill_indices_that_change_before_the_backward_pass():
+    """A change that autograd sees is refused. One that it does not see (a
+    storage written by another program) reaches no memory but the gradient."""
+    z = logits_of(4, 1003, torch.float32, "cuda", seed=1).requires_grad_()
+    values, indices, rest = answers(4, 1003, 6, torch.float32, "cuda", 1.0)
+    loss = O.distill_topk(z, values, indices, rest)
+    indices[1, 2] = 5
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss.sum(), z)
+    (want,) = torch.autograd.grad(O.distill_topk(z, values, indices, rest).sum(), z)
+    loss = O.distill_topk(z, values, indices, rest)
+    indices.data[2, 3] = 1003 + 17
+    indices.data[0, 0] = 2 ** 40
+    (grad,) = torch.autograd.grad(loss.sum(), z)
+    for row in (1, 3):
+        assert torch.equal(grad[row], want[row])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("vdtype", TYPES)
 def test_distill_types_of_the_answer(vdtype):
     z = logits_of(6, 301, torch.bfloat16, "cuda", seed=1)
