@@ -568,6 +568,33 @@ def test_offsets_beyond_32_bits():
 
 
 @pytest.mark.gpu
+def test_backward_offsets_beyond_32_bits():
+    """The backward pass makes offsets of its own: the gradients of equal images
+    are those of one alone, and the parameters' are as many times its sums."""
+    n, c, h, w = 9, 256, 1000, 1000
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    image, up = (torch.randn(1, h, w, c, device="cuda", generator=gen).bfloat16().permute(0, 3, 1, 2)
+                 for _ in range(2))
+    gn = nn.GroupNorm(32, c).cuda()
+    one = step(image, gn, "silu", up)
+    x = image.expand(n, c, h, w).contiguous(memory_format=torch.channels_last)
+    assert x.numel() > 2 ** 31
+    got = step(x, gn, "silu", up.expand(n, c, h, w))
+    # Nine images: a thread adds up 10^6 rows / 8 at a time / 228 chunks = 549
+    # values, then come 3 steps of joins, 228 chunks / 16 and 9 images: less than
+    # 600 roundings of 2^-24 of the sum of magnitudes. One image, in 2048 chunks:
+    # less than 150. |g| <= 1.1 |dy|, so a group's means of g and g h, with mean
+    # |g h| < 1, are within slack each, and |h| < 7 of a normal distribution.
+    slack = 768 * 2.0 ** -24
+    for i in (0, n // 2, n - 1):
+        off = (got["dx"][i].float() - one["dx"][0].float()).abs()
+        assert (off <= 2.0 ** -7 * one["dx"][0].float().abs() + 8 * slack).all()
+    size = (up[0].float() * image[0].float()).abs().sum((1, 2)) * 1.1
+    assert ((got["dweight"] - n * one["dweight"]).abs() <= slack * n * size).all()
+    assert ((got["dbias"] - n * one["dbias"]).abs() <= slack * n * 1.1 * up[0].float().abs().sum((1, 2))).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", ["efficientnet_b0", "resnet18"])
 def test_model_step_against_cpu(name):
     """A converted model's forward and gradients in fp32, GPU against CPU."""
