@@ -68,6 +68,10 @@ def load_checkpoint(model, checkpoint_path, use_ema=False, strict=True, ignore_k
             k: v for k, v in state_dict.items()
             if k in model_sd and model_sd[k].shape == v.shape
         }
+        missing = [k for k in model_sd if k not in state_dict]
+        if missing:
+            _logger.warning("%d of %d weights are not in '%s': %s ..", len(missing),
+                            len(model_sd), checkpoint_path, ", ".join(missing[:3]))
     model.load_state_dict(state_dict, strict=strict)
 
 

@@ -34,11 +34,14 @@ class InferenceEngine:
         self.dtype = torch.float16 if (fp16 and self.device == "cuda") else torch.float32
         model = create_deepfake_model_v4(
             model_name, num_classes=2, in_chans=12,
-            checkpoint_path=checkpoint, strict=False)
+            checkpoint_path="" if group_norm else checkpoint, strict=False)
         if group_norm:
+            from ..models.helpers import load_checkpoint
             from ..models.layers_extra import convert_groupnorm_model
 
             model = convert_groupnorm_model(model, group_norm)
+            if checkpoint:
+                load_checkpoint(model, checkpoint, strict=True)
         model = params.DeepFakeModel(model).to(self.device).to(self.dtype).eval()
         if self.device == "cuda":
             model = model.to(memory_format=torch.channels_last)

@@ -28,11 +28,14 @@ def test_img(img_paths, checkpoint_path="../models/model_half.pth.tar",
 
     basemodel = create_deepfake_model_v4(
         "efficientnet_deepfake_v4", num_classes=2, in_chans=12,
-        checkpoint_path=checkpoint_path, strict=False)
+        checkpoint_path="" if group_norm else checkpoint_path, strict=False)
     if group_norm:
+        from ..models.helpers import load_checkpoint
         from ..models.layers_extra import convert_groupnorm_model
 
         basemodel = convert_groupnorm_model(basemodel, group_norm)
+        if checkpoint_path:
+            load_checkpoint(basemodel, checkpoint_path, strict=True)
     model = DeepFakeModel(basemodel)
     model = model.to(device=device, dtype=dtype)
     if device == "cuda":
