@@ -222,8 +222,10 @@ def distill_topk(logits, values, indices, rest=None, temperature: float = 1.0):
     logits hold. An index beyond the classes makes its row's loss and gradient
     NaN. If two slots name one class, each has its own term in the loss and their
     probabilities add up in the gradient. A class at -inf has student probability
-    0; where the teacher gives it more, the loss is inf. The loss is not scaled
-    by temperature^2. Differentiable once, in
+    0; where the teacher gives it more, the loss is inf, as it is where a
+    logarithm of a probability is beyond fp32. Any finite logits and masks are
+    taken; a NaN or +inf among a row's logits leaves it no finite loss. The loss
+    is not scaled by temperature^2. Differentiable once, in
     logits; the teacher's answer is given. GPU: one pass over the logits
     forward, one backward (ops/hip/distill.hip).
     """

@@ -731,6 +731,28 @@ def finite_masks(device, dtype, mask, t, classes, check=check_distill):
         assert (off <= (torch.finfo(dtype).eps / 2 + U * (32 + 4 * size)) * want.abs() + least).all()
 
 
+def nothing_finite_from(device, classes):
+    for value in (float("nan"), INF):
+        for named in (True, False):
+            for with_rest in (True, False):
+                z = logits_of(3, classes, torch.float32, device, seed=1)
+                answer = answers(3, classes, 4, torch.float32, device, 1.0, with_rest)
+                other = next(i for i in range(classes) if i not in answer[1][1].tolist())
+                z[1, answer[1][1, 2] if named else other] = value
+                loss = O.distill_topk(z, *answer)
+                assert not loss[1].isfinite() and loss[[0, 2]].isfinite().all()
+
+
+def test_no_finite_loss_from_nan_or_inf_cpu():
+    nothing_finite_from("cpu", 203)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("classes", [9, 203, 20011])
+def test_no_finite_loss_from_nan_or_inf(classes):
+    nothing_finite_from("cuda", classes)
+
+
 MASKS = [-1e6, -1e9, -1e10, -1e12, -1e20, -1e25, -1e30, -3e38, 1e10, 1e20]
 
 
