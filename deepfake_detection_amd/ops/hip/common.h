@@ -1,6 +1,6 @@
 // Common helpers for the gfx950 (CDNA4) kernels.
 //
-// Conventions (per /opt/skills/guides/cdna_hip_programming.md):
+// Conventions:
 //   * wavefront = 64 lanes; blocks are multiples of 64
 //   * bf16/fp16 global access vectorized (>=8 B/lane)
 //   * memory-bound ops grid-stride with grid capped near 256 CU x 8 blocks
@@ -106,6 +106,31 @@ DFD_DEV DfdVec<T, N> dfd_vload(const T* p) {
 template <typename T, int N>
 DFD_DEV void dfd_vstore(T* p, const DfdVec<T, N>& x) {
   *reinterpret_cast<DfdVec<T, N>*>(p) = x;
+}
+
+// Loads and stores past the caches, which pays for tensors that they do not
+// hold: 16 byte vectors; narrower ones go as they are.
+template <typename T, int VEC>
+DFD_DEV DfdVec<T, VEC> dfd_vload_once(const T* p) {
+  if constexpr (VEC * sizeof(T) == 16) {
+    typedef unsigned Words __attribute__((ext_vector_type(4)));
+    const Words w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(p));
+    DfdVec<T, VEC> x;
+    __builtin_memcpy(&x, &w, sizeof(x));
+    return x;
+  } else {
+    return dfd_vload<T, VEC>(p);
+  }
+}
+
+template <typename T, int VEC>
+DFD_DEV void dfd_vstore_once(T* p, const DfdVec<T, VEC>& x) {
+  if constexpr (VEC * sizeof(T) == 16) {
+    typedef unsigned Words __attribute__((ext_vector_type(4)));
+    __builtin_nontemporal_store(*reinterpret_cast<const Words*>(&x), reinterpret_cast<Words*>(p));
+  } else {
+    dfd_vstore<T, VEC>(p, x);
+  }
 }
 
 // largest power-of-two vector width (≤16 B per lane) dividing C

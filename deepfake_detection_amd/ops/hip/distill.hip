@@ -92,15 +92,7 @@ struct Row {
   }
   DFD_DEV DfdVec<T, VEC> load(int v) const { return dfd_vload<T, VEC>(p + head + (long long)v * VEC); }
   DFD_DEV DfdVec<T, VEC> load_once(int v) const {
-    if constexpr (VEC * sizeof(T) == 16) {
-      typedef unsigned Words __attribute__((ext_vector_type(4)));
-      const Words w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(p + head + (long long)v * VEC));
-      DfdVec<T, VEC> x;
-      __builtin_memcpy(&x, &w, sizeof(x));
-      return x;
-    } else {
-      return load(v);
-    }
+    return dfd_vload_once<T, VEC>(p + head + (long long)v * VEC);
   }
   DFD_DEV int first(int v) const { return head + v * VEC; }
   DFD_DEV int edges() const { return head + tail; }
@@ -154,17 +146,6 @@ template <typename T, int VEC>
 DFD_DEV void to_floats(const DfdVec<T, VEC>& x, float (&z)[VEC]) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) z[i] = DfdCvt<T>::to_f32(x.v[i]);
-}
-
-// A store of what this op does not read again.
-template <typename T, int VEC>
-DFD_DEV void store_once(T* p, const DfdVec<T, VEC>& x) {
-  if constexpr (VEC * sizeof(T) == 16) {
-    typedef unsigned Words __attribute__((ext_vector_type(4)));
-    __builtin_nontemporal_store(*reinterpret_cast<const Words*>(&x), reinterpret_cast<Words*>(p));
-  } else {
-    dfd_vstore<T, VEC>(p, x);
-  }
 }
 
 // Order-preserving keys: any NaN is the largest, -0 and 0 are equal, and 0 is
@@ -666,7 +647,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(
     DfdVec<T, VEC> o;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) o.v[i] = of_rest(z[i]);
-    store_once<T, VEC>(out + row.first(v), o);
+    dfd_vstore_once<T, VEC>(out + row.first(v), o);
   });
   for (int e = tid; e < row.edges(); e += THREADS)
     out[row.edge(e)] = of_rest(row.at(row.edge(e)));

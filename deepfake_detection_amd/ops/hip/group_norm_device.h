@@ -352,31 +352,6 @@ DFD_DEV float gn_act_slope(float z, Act act) {
   }
 }
 
-// A load of what this op does not read again.
-template <typename T, int VEC>
-DFD_DEV DfdVec<T, VEC> gn_load_once(const T* p) {
-  if constexpr (VEC * sizeof(T) == 16) {
-    typedef unsigned Words __attribute__((ext_vector_type(4)));
-    const Words w = __builtin_nontemporal_load(reinterpret_cast<const Words*>(p));
-    DfdVec<T, VEC> x;
-    __builtin_memcpy(&x, &w, sizeof(x));
-    return x;
-  } else {
-    return dfd_vload<T, VEC>(p);
-  }
-}
-
-// A store past the caches: they keep what the pass reads again.
-template <typename T, int VEC>
-DFD_DEV void gn_store_once(T* p, const DfdVec<T, VEC>& x) {
-  if constexpr (VEC * sizeof(T) == 16) {
-    typedef unsigned Words __attribute__((ext_vector_type(4)));
-    __builtin_nontemporal_store(*reinterpret_cast<const Words*>(&x), reinterpret_cast<Words*>(p));
-  } else {
-    dfd_vstore<T, VEC>(p, x);
-  }
-}
-
 // The widest vector of channels, at most 16 bytes, that divides the channels
 // and that every tensor's address allows.
 static inline int gn_elem(GnType t) { return t == GnType::kF32 ? 4 : 2; }
