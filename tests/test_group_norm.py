@@ -616,3 +616,8 @@ def test_model_step_against_cpu(name):
     for k, p in model.named_parameters():
         a, b = p.grad.cpu(), grads[k]
         assert (a - b).norm() <= 5e-3 * b.norm() + 1e-5, k
+
+
+@pytest.mark.gpu
+def test_model_with_norms_of_pooled_features_against_cpu():
+    test_model_step_against_cpu("skresnet18")
